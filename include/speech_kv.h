@@ -440,6 +440,98 @@ SKV_API int skv_reduce_add_layernorm(const float* part, int32_t splits, const vo
                                      const void* gamma, const void* beta, float eps, void* sum, int64_t lds, void* norm,
                                      int64_t ldn, int32_t rows, int32_t hidden, int32_t dtype, void* stream);
 
+/*
+ * skv_append_rotary — skv_append with the position rotation on the way, q's rows rotated in the same launch.
+ *   y[i] = x[i] cos_i - x[i + r/2] sin_i and y[i + r/2] = x[i + r/2] cos_i + x[i] sin_i for i < r/2, r = rot_dim
+ *   (interleaved: the pairs are 2i, 2i + 1); dims from rot_dim on stay as they are. fp32 arithmetic, rounded to dtype once.
+ *   q, k_new, v_new : [N, heads, D] rows at their own strides (q_stride_n, q_stride_h, ...); q NULL: none
+ *   q_out, k_out    : where rotated rows go, [N, heads, D] at their own strides; q_out with q, and may be q; k_out may be
+ *                     k_new, or NULL (rotated keys then go to the pool alone)
+ *   positions : int64 [N]; cos_sin : fp32 [num_positions, rot_dim] contiguous, a row holding rot_dim / 2 cosines, then
+ *               the sines. A position outside the table: the row's K and V are not stored, its q_out and k_out are zeros.
+ *   pools, slot_mapping : as skv_append (a row whose slot is outside the pool is rotated and not stored; rows of one call
+ *               that name the same slot race)
+ *   head_dim and rot_dim multiples of two 16-byte vectors (16 elements; fp32: 8).
+ * No counterpart in the reference, whose models add absolute positions; it stands beside skv_append.
+ */
+SKV_API int skv_append_rotary(const void* q, int64_t q_stride_n, int64_t q_stride_h, const void* k_new,
+                              int64_t k_stride_n, int64_t k_stride_h, const void* v_new, int64_t v_stride_n,
+                              int64_t v_stride_h, void* q_out, int64_t qo_stride_n, int64_t qo_stride_h, void* k_out,
+                              int64_t ko_stride_n, int64_t ko_stride_h, void* k_pool, void* v_pool,
+                              const int64_t* slot_mapping, const int64_t* positions, const float* cos_sin,
+                              int64_t num_positions, int32_t rot_dim, int32_t interleaved, int32_t n_tokens,
+                              int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int64_t num_slots,
+                              int32_t dtype, void* stream);
+
+/*
+ * The 4-bit paged cache (skv_append_int4, skv_gather_int4, skv_paged_attention_int4): 5 bits an element.
+ *   Each 32 consecutive dims of a (token, head) row share fp16 (scale, low); an element is low + scale * code, code 0..15:
+ *   low = fp16(min), scale = fp16(max(0, (max - low) / 15)), code = round((x - low) * (1 / scale)) clamped (0 where scale
+ *   is 0), in fp32. Values beyond +-16384 saturate and a NaN is held as 0.
+ *   Pools: uint8 [num_blocks, kv heads, block_size / 16, 10 * D], block_size a multiple of 16, D in {32, 64, 128}. The
+ *   16-token tile of a K pool is [16 tokens][D / 2] bytes, a dword per 8 dims with dims 0..7 in nibbles 0, 4, 1, 5, 2, 6, 3,
+ *   7, then [16][D / 32] fp16 pairs (scale, low); of a V pool [4 quads][D / 2][4 tokens] bytes, dims 2m and 2m + 1 in the low
+ *   and high nibble of byte m, then [4 quads][D / 32][scale, low][4 tokens in the order 0, 2, 1, 3] fp16.
+ *   No counterpart in the reference, whose pools are 16-bit.
+ *
+ * skv_append_int4 — K/V rows quantised into their slots, rotated first when cos_sin is given (then as skv_append_rotary, q,
+ *   q_out and k_out included; the codes are those of the rotated row rounded to dtype). cos_sin NULL: no rotation, and
+ *   q, q_out, k_out, positions NULL. rot_dim a multiple of 16. Rows of one call that name the same slot leave a mixture of
+ *   them there.
+ */
+SKV_API int skv_append_int4(const void* q, int64_t q_stride_n, int64_t q_stride_h, const void* k_new, int64_t k_stride_n,
+                            int64_t k_stride_h, const void* v_new, int64_t v_stride_n, int64_t v_stride_h, void* q_out,
+                            int64_t qo_stride_n, int64_t qo_stride_h, void* k_out, int64_t ko_stride_n,
+                            int64_t ko_stride_h, void* k_pool, void* v_pool, const int64_t* slot_mapping,
+                            const int64_t* positions, const float* cos_sin, int64_t num_positions, int32_t rot_dim,
+                            int32_t interleaved, int32_t n_tokens, int32_t num_heads, int32_t num_kv_heads,
+                            int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t dtype, void* stream);
+
+/*
+ * skv_gather_int4 — skv_gather from 4-bit pools: the values in dtype, [B, kv heads, max_len, D] contiguous, zeros from
+ * lens[b] on and behind a block id outside the pool. max_len at most table_stride * block_size.
+ */
+SKV_API int skv_gather_int4(const void* k_pool, const void* v_pool, const int32_t* block_tables, int32_t table_stride,
+                            const int32_t* lens, void* k_out, void* v_out, int32_t batch, int32_t num_kv_heads,
+                            int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t max_len, int32_t dtype,
+                            void* stream);
+
+/* Key chunk that skv_paged_attention_int4 takes when chunk_tokens == 0 (a multiple of 64), and the workspace bytes of
+ * a call with a given chunk (0: none needed): one (max, sum, acc[head_dim]) fp32 partial per (query, head, chunk). */
+SKV_API int32_t skv_int4_chunk_tokens(int32_t batch, int32_t q_len, int32_t num_heads, int32_t num_kv_heads,
+                                      int32_t head_dim, int32_t max_ctx, int32_t dtype);
+SKV_API int64_t skv_int4_workspace_bytes(int32_t batch, int32_t q_len, int32_t num_heads, int32_t head_dim,
+                                         int32_t max_ctx, int32_t chunk_tokens);
+
+/*
+ * skv_paged_attention_int4 — softmax(q K^T * scale) V over the 4-bit paged cache of each row: skv_paged_attention's q, out,
+ * tables, ctx_lens, max_ctx and causal (0 or SKV_ATTN_CAUSAL), without a fused append. q and out are in dtype. A query with
+ * no visible key gets zeros; keys behind a block id outside the pool are left out. workspace: skv_int4_workspace_bytes, any
+ * content; two launches that may overlap in time need one each.
+ */
+SKV_API int skv_paged_attention_int4(const void* q, int64_t q_stride_b, int64_t q_stride_q, int64_t q_stride_h,
+                                     const void* k_pool, const void* v_pool, const int32_t* block_tables,
+                                     int32_t table_stride, const int32_t* table_rows, const int32_t* ctx_lens, void* out,
+                                     int64_t o_stride_b, int64_t o_stride_q, int64_t o_stride_h, int32_t batch,
+                                     int32_t q_len, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                     int32_t block_size, int32_t num_blocks, int32_t max_ctx, float scale, int32_t causal,
+                                     int32_t dtype, int32_t chunk_tokens, void* workspace, int64_t workspace_bytes,
+                                     void* stream);
+
+/*
+ * skv_prompt_attention — causal attention of packed prompts over their own keys.
+ *   q, out [N, num_heads, D], k, v [N, num_kv_heads, D] rows at their own strides (slices of a fused projection are fine);
+ *   sequence s is rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (int32 [num_seqs + 1] device, non-decreasing, within
+ *   0..N), of any length, 0 included; its query i sees its keys 0..i, whatever the later keys hold. Rows of out that belong
+ *   to no sequence are left as they are. head_dim in {16, 32, 64, 128}.
+ * Replaces, for prompts of different lengths, the padded batch of models.py:126-165.
+ */
+SKV_API int skv_prompt_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h, const void* k, int64_t k_stride_n,
+                                 int64_t k_stride_h, const void* v, int64_t v_stride_n, int64_t v_stride_h,
+                                 const int32_t* cu_seqlens, void* out, int64_t o_stride_n, int64_t o_stride_h,
+                                 int32_t n_tokens, int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                 int32_t head_dim, float scale, int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

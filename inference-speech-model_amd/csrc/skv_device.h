@@ -230,6 +230,19 @@ template <> __device__ __forceinline__ uint4 pack16<SKV_BF16>(const float* a) {
   return r;
 }
 
+// Division by a launch-constant divisor d without a divide: m = floor(2^32 / d)
+// (2^32 - 1 for d = 1), so umulhi(n, m) is floor(n / d) or one less for every
+// n < 2^32, and one remainder test corrects it.
+struct DivU32 {
+  uint32_t d, m;
+};
+inline DivU32 make_div(uint32_t d) { return {d, d == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / d)}; }
+__device__ __forceinline__ uint32_t udiv(uint32_t n, DivU32 f) {
+  uint32_t q = __umulhi(n, f.m);
+  if (n - q * f.d >= f.d) ++q;
+  return q;
+}
+
 __device__ __forceinline__ int lane_id() {
   return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
 }

@@ -87,19 +87,6 @@ namespace {
 // Loads and stores carry the nontemporal hint: at the encoder-store size (64 x 1500
 // rows of 20 x 64 bf16 per K and V) that is 2.5% faster than the default policy.
 // ---------------------------------------------------------------------------
-// Division by a launch-constant divisor d without a divide: m = floor(2^32 / d)
-// (2^32 - 1 for d = 1), so umulhi(n, m) is floor(n / d) or one less for every
-// n < 2^32, and one remainder test corrects it.
-struct DivU32 {
-  uint32_t d, m;
-};
-DivU32 make_div(uint32_t d) { return {d, d == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / d)}; }
-__device__ __forceinline__ uint32_t udiv(uint32_t n, DivU32 f) {
-  uint32_t q = __umulhi(n, f.m);
-  if (n - q * f.d >= f.d) ++q;
-  return q;
-}
-
 // Append with 32-bit element indices (total rows * heads * vectors < 2^31).
 __global__ __launch_bounds__(256) void append32_kernel(const uint4* __restrict__ k_new, const uint4* __restrict__ v_new,
                                                        int64_t sn, int64_t sh, uint4* __restrict__ k_pool,

@@ -16,6 +16,9 @@ Functions:
     decode_linear_residual(x, weight, bias, res), decode_linear_normed(x, stats, gamma, beta, eps, weight, ...)
                               (with the residual add behind, or the LayerNorm ahead)
     rows_linear(x, weight, bias, gelu, res), rows_qkv(x, weight, heads)   (many 16-bit rows)
+    append_rotary(k_new, v_new, k_pool, v_pool, slot_mapping, positions, cos_sin, q, ...), rotary_table(...)
+    prompt_attention(q, k, v, cu_seqlens, scale)   (causal, packed prompts)
+    append_int4(...), gather_int4(...), paged_attention_int4(...), int4_pool_shape(...)   (the 4-bit paged cache)
 """
 from __future__ import annotations
 
@@ -71,6 +74,17 @@ SIGNATURES = {
                                          _c_p, _c_i64, _c_p, _c_i32, _c_i32, _c_i32, _c_i32, _c_p]),
     "skv_rows_linear": (_c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i32, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i32,
                                  _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_p]),
+    "skv_append_rotary": (_c_int, [_c_p, _c_i64, _c_i64] * 5 + [_c_p] * 5 + [_c_i64] + [_c_i32] * 6 +
+                          [_c_i64, _c_i32, _c_p]),
+    "skv_append_int4": (_c_int, [_c_p, _c_i64, _c_i64] * 5 + [_c_p] * 5 + [_c_i64] + [_c_i32] * 9 + [_c_p]),
+    "skv_gather_int4": (_c_int, [_c_p, _c_p, _c_p, _c_i32, _c_p, _c_p, _c_p] + [_c_i32] * 7 + [_c_p]),
+    "skv_int4_chunk_tokens": (_c_i32, [_c_i32] * 7),
+    "skv_int4_workspace_bytes": (_c_i64, [_c_i32] * 6),
+    "skv_paged_attention_int4": (_c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i32, _c_p, _c_p, _c_p, _c_i64,
+                                          _c_i64, _c_i64] + [_c_i32] * 8 + [_c_f, _c_i32, _c_i32, _c_i32, _c_p, _c_i64,
+                                                                           _c_p]),
+    "skv_prompt_attention": (_c_int, [_c_p, _c_i64, _c_i64] * 3 + [_c_p, _c_p, _c_i64, _c_i64] + [_c_i32] * 5 +
+                             [_c_f, _c_i32, _c_p]),
     "skv_decode_linear_splits": (_c_i32, [_c_i32, _c_i32]),
     "skv_decode_linear_partials": (_c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
                                             _c_p]),
@@ -1001,4 +1015,287 @@ def codebook_embed_sum(codes: torch.Tensor, tables: Sequence[torch.Tensor]) -> t
     rc = lib().skv_codebook_embed_sum(c2.data_ptr(), c2.stride(0) if rows > 1 else k, rows, ptrs, k, vocab, dim,
                                       out.data_ptr(), dim, _code(dt), _stream(codes.device))
     _check(rc, "skv_codebook_embed_sum")
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions, packed prompts, the 4-bit paged cache.
+# ---------------------------------------------------------------------------
+INT4_HEAD_DIMS = (32, 64, 128)
+INT4_TILE = 16  # tokens of a tile (kTile of the library)
+
+
+def _one_device(what: str, *named: Tuple[str, Optional[torch.Tensor]]) -> int:
+    """The GPU that all the given tensors are on; RuntimeError when they are not on one."""
+    dev = -1
+    for name, t in named:
+        if t is None:
+            continue
+        idx = t.get_device()
+        if idx < 0:
+            _gpu(t, name)
+        if dev < 0:
+            dev = idx
+        elif idx != dev:
+            raise RuntimeError(f"{what}: {name} is on GPU {idx}, the other tensors on GPU {dev}")
+    return dev
+
+
+def _call(what: str, dev: int, *args) -> None:
+    """One library call on the current stream of GPU `dev`, which is made the current device for it."""
+    fn = getattr(lib(), what)
+    if dev == torch.cuda.current_device():
+        _check(fn(*args, _stream(torch.device("cuda", dev))), what)
+    else:
+        with torch.cuda.device(dev):
+            _check(fn(*args, _stream(torch.device("cuda", dev))), what)
+
+
+def _rows3(what: str, t: torch.Tensor, name: str, shape: Tuple[int, int, int], dtype: torch.dtype,
+           written: bool = False) -> torch.Tensor:
+    """t as [N, H, D] rows with contiguous, 16-byte aligned vectors: a copy where an input is laid out otherwise, RuntimeError
+    where an output is (or where its rows overlap)."""
+    if tuple(t.shape) != shape or t.dtype != dtype:
+        raise RuntimeError(f"{what}: {name} must be {list(shape)} {dtype}, got {list(t.shape)} {t.dtype}")
+    epl = 16 // t.element_size()
+    sn, sh, sd = t.stride()
+    ok = (sd == 1 or shape[2] == 1) and sn % epl == 0 and sh % epl == 0 and t.data_ptr() % 16 == 0
+    if written:
+        n, h, d = shape
+        if ok and n > 1 and h > 1:
+            ok = sh >= d and sn >= (h - 1) * sh + d or sn >= d and sh >= (n - 1) * sn + d
+        elif ok and (n > 1 or h > 1):
+            ok = (sn if n > 1 else sh) >= d
+        if not ok:
+            raise RuntimeError(f"{what}: {name} must have a contiguous last dim, 16-byte aligned rows and no overlap")
+    return t if ok else t.contiguous()
+
+
+def rotary_table(max_positions: int, rot_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
+    """The cos_sin table [max_positions, rot_dim] of append_rotary: the cosines of position * base^(-2 i / rot_dim), i <
+    rot_dim / 2, then the sines. Angles in float64 (at position 100000 a float32 angle is off by up to 4e-3), stored in float32."""
+    if max_positions < 0 or rot_dim <= 0 or rot_dim % 2:
+        raise RuntimeError(f"rotary_table: {max_positions} positions, rot_dim {rot_dim} (positive and even)")
+    freq = float(base) ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / rot_dim)
+    ang = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat([ang.cos(), ang.sin()], dim=1).to(torch.float32)
+
+
+def _index64(what: str, t: torch.Tensor, name: str, n: int) -> torch.Tensor:
+    if t.dtype != torch.int64 or t.numel() != n:
+        raise RuntimeError(f"{what}: {name} must be int64 [{n}], got {t.dtype} {list(t.shape)}")
+    return t.contiguous()
+
+
+def _append_rows(what: str, k_new, v_new, slot_mapping, positions, cos_sin, q, q_out, k_out):
+    """(device, the argument list of a rotating append up to its pools, q_out, what keeps the arguments alive)."""
+    if k_new.dim() != 3:
+        raise RuntimeError(f"{what}: k_new must be [N, H, D], got {list(k_new.shape)}")
+    dev = _one_device(what, ("k_new", k_new), ("v_new", v_new), ("slot_mapping", slot_mapping), ("positions", positions),
+                      ("cos_sin", cos_sin), ("q", q), ("q_out", q_out), ("k_out", k_out))
+    n, h, d = k_new.shape
+    dt = k_new.dtype
+    _code(dt)
+    k_new = _rows3(what, k_new, "k_new", (n, h, d), dt)
+    v_new = _rows3(what, v_new, "v_new", (n, h, d), dt)
+    slot_mapping = _index64(what, slot_mapping, "slot_mapping", n)
+    if (cos_sin is None) != (positions is None):
+        raise RuntimeError(f"{what}: positions and cos_sin go together")
+    if cos_sin is None and (q is not None or k_out is not None):
+        raise RuntimeError(f"{what}: q and k_out come with positions and cos_sin")
+    if q is None and q_out is not None:
+        raise RuntimeError(f"{what}: q_out comes with q")
+    if cos_sin is not None:
+        positions = _index64(what, positions, "positions", n)
+        if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous():
+            raise RuntimeError(f"{what}: cos_sin must be contiguous float32 [positions, rot_dim]")
+    args = []
+    if q is not None:
+        if q.dim() != 3:
+            raise RuntimeError(f"{what}: q must be [N, heads, D], got {list(q.shape)}")
+        q = _rows3(what, q, "q", (n, q.shape[1], d), dt)
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=dt, device=q.device)
+        else:
+            q_out = _rows3(what, q_out, "q_out", tuple(q.shape), dt, written=True)
+    if k_out is not None:
+        k_out = _rows3(what, k_out, "k_out", (n, h, d), dt, written=True)
+    for t in (q, k_new, v_new, q_out, k_out):
+        args += [None, 0, 0] if t is None else [t.data_ptr(), t.stride(0), t.stride(1)]
+    return dev, args, q_out, (q, k_new, v_new, slot_mapping, positions)
+
+
+def append_rotary(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                  slot_mapping: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                  q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
+                  k_out: Optional[torch.Tensor] = None, interleaved: bool = False) -> Optional[torch.Tensor]:
+    """append() with the position rotation on the way: pool[slot] = rotated k row and v row; returns the rotated q rows.
+
+    k_new, v_new: [N, Hkv, D]; q: [N, H, D] (any row/head strides, so slices of a fused projection are fine).
+    positions: int64 [N]; cos_sin: rotary_table(...) [max_positions, rot_dim], rot_dim <= D: the first rot_dim dims turn, in
+    pairs (i, i + rot_dim / 2), with interleaved (2i, 2i + 1); fp32 arithmetic, rounded once.
+    q_out (may be q), k_out (may be k_new): where the rotated rows go; without k_out the keys go to the pool alone.
+    A negative slot skips the row's store. A position outside the table skips it too and leaves zeros in q_out and k_out.
+    """
+    what = "append_rotary"
+    if cos_sin is None or positions is None:
+        raise RuntimeError(f"{what}: positions and cos_sin are required (append() stores rows as they are)")
+    dev, args, q_out, keep = _append_rows(what, k_new, v_new, slot_mapping, positions, cos_sin, q, q_out, k_out)
+    n, h, d = k_new.shape
+    for t, name in ((k_pool, "k_pool"), (v_pool, "v_pool")):
+        if t.dim() != 4 or t.shape[2:] != (h, d) or t.shape != k_pool.shape or t.dtype != k_new.dtype or \
+                not t.is_contiguous() or t.get_device() != dev:
+            raise RuntimeError(f"{what}: {name} must be contiguous [num_blocks, block_size, {h}, {d}] {k_new.dtype} on the "
+                               f"rows' GPU, got {list(t.shape)} {t.dtype}")
+    _call("skv_append_rotary", dev, *args, k_pool.data_ptr(), v_pool.data_ptr(), keep[3].data_ptr(), keep[4].data_ptr(),
+          cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[1], 1 if interleaved else 0, n,
+          0 if q is None else q.shape[1], h, d, k_pool.shape[0] * k_pool.shape[1], _code(k_new.dtype))
+    return q_out
+
+
+def int4_pool_shape(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int) -> Tuple[int, int, int, int]:
+    """Shape of a uint8 K or V pool of the 4-bit cache (see speech_kv.h): 5 bits an element."""
+    if head_dim not in INT4_HEAD_DIMS or block_size <= 0 or block_size % INT4_TILE:
+        raise RuntimeError(f"int4_pool_shape: head_dim {head_dim} (one of {INT4_HEAD_DIMS}), block_size {block_size} "
+                           f"(a multiple of {INT4_TILE})")
+    return num_blocks, num_kv_heads, block_size // INT4_TILE, 10 * head_dim
+
+
+def _int4_pools(what: str, k_pool: torch.Tensor, v_pool: torch.Tensor) -> Tuple[int, int, int, int]:
+    """(num_blocks, block_size, kv heads, head_dim) of a pair of 4-bit pools."""
+    for t, name in ((k_pool, "k_pool"), (v_pool, "v_pool")):
+        if t.dim() != 4 or t.dtype != torch.uint8 or not t.is_contiguous() or t.shape != k_pool.shape or t.shape[3] % 10:
+            raise RuntimeError(f"{what}: {name} must be contiguous uint8 [num_blocks, kv heads, block_size / 16, 10 * D], "
+                               f"got {list(t.shape)} {t.dtype}")
+    nb, h, tiles, w = k_pool.shape
+    return nb, tiles * INT4_TILE, h, w // 10
+
+
+def append_int4(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                slot_mapping: torch.Tensor, positions: Optional[torch.Tensor] = None,
+                cos_sin: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
+                q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+                interleaved: bool = False) -> Optional[torch.Tensor]:
+    """append() into 4-bit pools (int4_pool_shape, uint8): the rows are quantised, each 32 dims to 16 levels between their
+    least and greatest value. With positions and cos_sin the keys (and q, whose rotated rows are returned) are rotated first,
+    as append_rotary does; the codes are those of the rotated row rounded to the rows' type."""
+    what = "append_int4"
+    dev, args, q_out, keep = _append_rows(what, k_new, v_new, slot_mapping, positions, cos_sin, q, q_out, k_out)
+    nb, bs, hp, dp = _int4_pools(what, k_pool, v_pool)
+    n, h, d = k_new.shape
+    if (hp, dp) != (h, d) or k_pool.get_device() != dev or v_pool.get_device() != dev:
+        raise RuntimeError(f"{what}: pools of {hp} heads x {dp} do not fit rows [*, {h}, {d}], or are on another GPU")
+    _call("skv_append_int4", dev, *args, k_pool.data_ptr(), v_pool.data_ptr(), keep[3].data_ptr(), _ptr(keep[4]),
+          _ptr(cos_sin), 0 if cos_sin is None else cos_sin.shape[0], 0 if cos_sin is None else cos_sin.shape[1],
+          1 if interleaved else 0, n, 0 if q is None else q.shape[1], h, d, bs, nb, _code(k_new.dtype))
+    return q_out
+
+
+def gather_int4(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor, lens: torch.Tensor, max_len: int,
+                dtype: torch.dtype, k_out: Optional[torch.Tensor] = None,
+                v_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """gather() from 4-bit pools: the values they hold as contiguous [B, H, max_len, D] of dtype, zero beyond lens[b]."""
+    what = "gather_int4"
+    block_tables, lens = _i32(block_tables, "block_tables"), _i32(lens, "lens")
+    dev = _one_device(what, ("k_pool", k_pool), ("v_pool", v_pool), ("block_tables", block_tables), ("lens", lens),
+                      ("k_out", k_out), ("v_out", v_out))
+    nb, bs, h, d = _int4_pools(what, k_pool, v_pool)
+    if block_tables.dim() != 2 or lens.numel() < block_tables.shape[0]:
+        raise RuntimeError(f"{what}: block_tables must be [B, max_blocks] and lens must cover the rows")
+    b = block_tables.shape[0]
+    if not 0 <= max_len <= block_tables.shape[1] * bs:
+        raise RuntimeError(f"{what}: max_len {max_len} outside the table's {block_tables.shape[1] * bs} positions")
+    code = _code(dtype)
+    outs = []
+    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
+        if t is None:
+            t = torch.empty((b, h, max_len, d), dtype=dtype, device=k_pool.device)
+        elif tuple(t.shape) != (b, h, max_len, d) or t.dtype != dtype or not t.is_contiguous():
+            raise RuntimeError(f"{what}: {name} must be contiguous [{b}, {h}, {max_len}, {d}] {dtype}")
+        outs.append(t)
+    _call("skv_gather_int4", dev, k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(), block_tables.shape[1],
+          lens.data_ptr(), outs[0].data_ptr(), outs[1].data_ptr(), b, h, d, bs, nb, int(max_len), code)
+    return outs[0], outs[1]
+
+
+@functools.lru_cache(maxsize=4096)
+def _int4_plan(batch: int, q_len: int, heads: int, kv_heads: int, head_dim: int, max_ctx: int, code: int,
+               chunk: int) -> Tuple[int, int]:
+    if chunk <= 0:
+        chunk = int(lib().skv_int4_chunk_tokens(batch, q_len, heads, kv_heads, head_dim, max_ctx, code))
+    return chunk, int(lib().skv_int4_workspace_bytes(batch, q_len, heads, head_dim, max_ctx, chunk))
+
+
+def paged_attention_int4(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor,
+                         ctx_lens: torch.Tensor, max_ctx: int, scale: float, causal: bool = False,
+                         table_rows: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                         chunk_tokens: int = 0) -> torch.Tensor:
+    """paged_attention() over a 4-bit cache: softmax(q K^T * scale) V over the values that each row's blocks hold.
+
+    q: [B, H, D] or [B, Q, H, D] in any of the three types, which is the result's; the other arguments are
+    paged_attention's. The split-K partials live in memory of this call's own, so captured graphs share none."""
+    what = "paged_attention_int4"
+    block_tables, ctx_lens = _i32(block_tables, "block_tables"), _i32(ctx_lens, "ctx_lens")
+    if table_rows is not None:
+        table_rows = _i32(table_rows, "table_rows")
+    dev = _one_device(what, ("q", q), ("k_pool", k_pool), ("v_pool", v_pool), ("block_tables", block_tables),
+                      ("ctx_lens", ctx_lens), ("table_rows", table_rows), ("out", out))
+    nb, bs, hkv, dk = _int4_pools(what, k_pool, v_pool)
+    q4 = _q4(q, "q")
+    bsz, qlen, heads, d = q4.shape
+    if d != dk or heads % hkv:
+        raise RuntimeError(f"{what}: {heads} heads x {d} do not fit pools of {hkv} heads x {dk}")
+    if block_tables.dim() != 2 or ctx_lens.numel() < bsz:
+        raise RuntimeError(f"{what}: block_tables must be 2-D and ctx_lens must cover the batch")
+    if table_rows is None and block_tables.shape[0] < bsz:
+        raise RuntimeError(f"{what}: {block_tables.shape[0]} table rows for batch {bsz}")
+    if table_rows is not None and table_rows.numel() < bsz:
+        raise RuntimeError(f"{what}: table_rows must cover the batch")
+    code = _code(q.dtype)
+    epl = 16 // q.element_size()
+    if q4.stride(3) != 1 or q4.data_ptr() % 16 or any(st % epl for st in q4.stride()[:3]):
+        q4 = q4.contiguous()
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    o4 = _q4(out, "out")
+    if tuple(o4.shape) != tuple(q4.shape) or o4.stride(3) != 1 or out.dtype != q.dtype:
+        raise RuntimeError(f"{what}: out must match q's shape and type with contiguous head_dim")
+    max_ctx = max(0, min(int(max_ctx), block_tables.shape[1] * bs))
+    chunk, need = _int4_plan(bsz, qlen, heads, hkv, d, max_ctx, code, int(chunk_tokens))
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _call("skv_paged_attention_int4", dev, q4.data_ptr(), q4.stride(0), q4.stride(1), q4.stride(2), k_pool.data_ptr(),
+          v_pool.data_ptr(), block_tables.data_ptr(), block_tables.shape[1], _ptr(table_rows), ctx_lens.data_ptr(),
+          o4.data_ptr(), o4.stride(0), o4.stride(1), o4.stride(2), bsz, qlen, heads, hkv, d, bs, nb, max_ctx, float(scale),
+          SKV_ATTN_CAUSAL if causal else 0, code, chunk, _ptr(ws), need)
+    return out
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal softmax(q K^T * scale) V of packed prompts: sequence s is rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1, and its
+    query i sees its keys 0..i.
+
+    q: [N, H, D]; k, v: [N, Hkv, D], H a multiple of Hkv (any row/head strides); cu_seqlens: int32 [S + 1] on the GPU. Rows of
+    out behind the last sequence (a padded batch) are left as they are; they are undefined when out is not given.
+    Reference math: speech_serving/models.py:126-165, per prompt."""
+    what = "prompt_attention"
+    cu_seqlens = _i32(cu_seqlens, "cu_seqlens")
+    dev = _one_device(what, ("q", q), ("k", k), ("v", v), ("cu_seqlens", cu_seqlens), ("out", out))
+    if q.dim() != 3 or k.dim() != 3:
+        raise RuntimeError(f"{what}: q, k, v must be [N, heads, D], got {list(q.shape)}, {list(k.shape)}")
+    n, heads, d = q.shape
+    hkv = k.shape[1]
+    if cu_seqlens.numel() < 1 or hkv == 0 or heads % hkv:
+        raise RuntimeError(f"{what}: cu_seqlens must hold at least one entry, {heads} heads must be a multiple of {hkv}")
+    code = _code(q.dtype)
+    q = _rows3(what, q, "q", (n, heads, d), q.dtype)
+    k = _rows3(what, k, "k", (n, hkv, d), q.dtype)
+    v = _rows3(what, v, "v", (n, hkv, d), q.dtype)
+    if out is None:
+        out = torch.empty((n, heads, d), dtype=q.dtype, device=q.device)
+    else:
+        _rows3(what, out, "out", (n, heads, d), q.dtype, written=True)
+    _call("skv_prompt_attention", dev, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+          v.data_ptr(), v.stride(0), v.stride(1), cu_seqlens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), n,
+          cu_seqlens.numel() - 1, heads, hkv, d, float(scale), code)
     return out
