@@ -14,6 +14,8 @@
 // hold neighbouring dims, those of a V dword tokens 0, 2 and 1, 3 of one dim.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "skv_common.h"
 #include "skv_rotary.h"
 
@@ -270,15 +272,20 @@ struct Int4Attn {
 constexpr int kPad = 4;  // floats (max, sum, unused) ahead of a partial's accumulators
 constexpr int kAttnWaves = 4;
 
+// A wave-uniform word of a table that the kernel does not write: a scalar load.
+__device__ __forceinline__ int32_t scalar_word(const int32_t* p) {
+  return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
+}
+
 // Keys query qi of row b sees.
 __device__ __forceinline__ int visible(const Int4Attn& p, int b, int qi) {
-  const int len = p.lens[b] - (p.causal ? p.qlen - 1 - qi : 0);
+  const int len = scalar_word(p.lens + b) - (p.causal ? p.qlen - 1 - qi : 0);
   return min(max(len, 0), p.max_ctx);
 }
 
 // One workgroup per (row, query, head, key chunk), everything in fp32: 16-key tiles go to its waves in turn.
 // Scores: lane (g, r) takes a quarter of key r's dims. Values: lane m takes dims 2m and 2m + 1 of D / 2 lanes' worth of
-// quads. The simple form, for fp32 rows.
+// quads. For fp32 rows, whose results are held to fp32's rounding.
 template <int DT, int D>
 __global__ __launch_bounds__(64 * kAttnWaves) void attention_int4_kernel(Int4Attn p) {
   constexpr int ND = D / 32;        // dwords of a lane's quarter row
@@ -306,12 +313,9 @@ __global__ __launch_bounds__(64 * kAttnWaves) void attention_int4_kernel(Int4Att
     for (int e = 0; e < 8; ++e) s_q[8 * threadIdx.x + e] = f[e];
   }
   __syncthreads();
-  float qf[8 * ND], qsum = 0.f;
+  float qf[8 * ND];
 #pragma unroll
-  for (int e = 0; e < 8 * ND; ++e) {
-    qf[e] = s_q[g * 8 * ND + e];
-    qsum += qf[e];
-  }
+  for (int e = 0; e < 8 * ND; ++e) qf[e] = s_q[g * 8 * ND + e];
   const int32_t* trow = p.tables + (int64_t)(p.trows ? p.trows[b] : b) * p.tstride;
   const int m = lane % LPM, part = lane / LPM;
   float top = kNegInf, sum = 0.f, a0 = 0.f, a1 = 0.f;
@@ -322,17 +326,17 @@ __global__ __launch_bounds__(64 * kAttnWaves) void attention_int4_kernel(Int4Att
     const int64_t at = (((int64_t)blk * p.kv_heads + kvh) * p.tiles + tile % p.tiles) * (10 * D);
     const char *kt = p.k_pool + at, *vt = p.v_pool + at;
     float s = 0.f;
+    const uint32_t km = *reinterpret_cast<const uint32_t*>(kt + 8 * D + (r * (D / kGroup) + g * 8 * ND / kGroup) * 4);
+    const float k_scale = half_bits(km & 0xffffu), k_low = half_bits(km >> 16);
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
       const uint32_t w = *reinterpret_cast<const uint32_t*>(kt + r * (D / 2) + (g * ND + i) * 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s = fmaf(qf[8 * i + 2 * e], (float)((w >> (4 * e)) & 15u), s);
-        s = fmaf(qf[8 * i + 2 * e + 1], (float)((w >> (4 * e + 16)) & 15u), s);
+        s = fmaf(qf[8 * i + 2 * e], fmaf(k_scale, (float)((w >> (4 * e)) & 15u), k_low), s);
+        s = fmaf(qf[8 * i + 2 * e + 1], fmaf(k_scale, (float)((w >> (4 * e + 16)) & 15u), k_low), s);
       }
     }
-    const uint32_t km = *reinterpret_cast<const uint32_t*>(kt + 8 * D + (r * (D / kGroup) + g * 8 * ND / kGroup) * 4);
-    s = fmaf(s, half_bits(km & 0xffffu), qsum * half_bits(km >> 16));
     s += xor_lane<16>(s);
     s += xor_lane<32>(s);
     s = t0 + r < t_end ? s * p.scale_log2 : kNegInf;
@@ -409,32 +413,480 @@ __global__ __launch_bounds__(64 * kAttnWaves) void attention_int4_kernel(Int4Att
     reinterpret_cast<uint16_t*>(o)[d] = (uint16_t)pack2<DT>(out, 0.f);
 }
 
-// Rows of several chunks: one workgroup of D threads per (row, query, head) joins the chunks' partials.
+// 16-bit rows on the matrix cores. One workgroup per (row, KV head, 16 queries, key chunk): the queries are those of the
+// head's whole group, so its keys are read once for all of them; its waves take 32-key steps in turn and join at the end.
+// Codes become fp16 in two operations: shifted and masked under the exponent of 16 they are 16 + code exactly.
+//   S^T = K Q^T: lane (g, r) unpacks 8 dims of key r, the operand of one product per 32 dims that share a scale, whose
+//     results (keys 4 g + i of query r) take that scale in fp32; it reaches them from the lane of the 16 that loaded it. One
+//     more product adds low and takes off 16 scale, against the sums of q over each 32 dims: K is exact.
+//   O^T = V^T P^T: the lane's 8 weights are the operand P^T (keys 4 g + 0, 2, 1, 3 of both tiles), and it unpacks those keys'
+//     dims [r D / 16, + D / 16) of V, one operand per dim. There the scale belongs to the contraction, so V's own operand takes
+//     it: scale * (16 + code) + z in one fma, z = fp16(-24 scale), is the value about the group's middle, rounded once (2^-11
+//     of it, what a cache in fp16 rounds too). The rest, low - 16 scale - z, is the group's own and one product more.
+// Both products run in fp16 whatever the rows' type: queries are first scaled by a power of two that brings their greatest
+// element to [0.5, 1), which the scores' factor takes back. Weights (times 2^6, clear of fp16's subnormals) go in as a
+// rounded head and its rounded remainder; their sum is one more row of the product.
+// fp16, 300 keys: 2.7e-4 of the results' rms from float64, where rounding exact ones is 2.1e-4 (with K's scale in its operand
+// as well 3.6e-4, with weights rounded once 3.3e-4, with low - 16 scale rounded into the fma 25e-4).
+// What bounds it: HBM for long rows, with about 2.2 vector operations an element beside them.
+constexpr float kLazyMaxLog2 = 8.f;  // the accumulators are rescaled when a maximum grows by more than this
+constexpr float kWeightLog2 = 6.f;   // weights below 2^(8 + 6)
+
+__device__ __forceinline__ uint32_t pk_fma(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2v, a), __builtin_bit_cast(half2v, b),
+                                                                __builtin_bit_cast(half2v, c)));
+}
+// 16 + code of nibbles K and K + 4 of w. mask and base are kCodeMask and kCodeBase in registers, which lets one instruction
+// do both.
+constexpr uint32_t kCodeMask = 0x03c003c0u, kCodeBase = 0x4c004c00u;
+template <int K>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t mask, uint32_t base) {
+  const uint32_t x = K == 0 ? w << 6 : (K == 1 ? w << 2 : (K == 2 ? w >> 2 : w >> 6));
+  return (x & mask) | base;
+}
+// All 8 codes of w with one shift, for a product that can take off different bases: 1024 + code of dims 0, 1, 4, 5 (nibbles 0,
+// 4, 2, 6), 64 + code of dims 2, 3, 6, 7.
+struct CodeRegs {
+  uint32_t low, base_low, high, base_high;
+};
+__device__ __forceinline__ uint4 code_row(uint32_t w, const CodeRegs& c) {
+  const uint32_t x = w >> 8;
+  return make_uint4((w & c.low) | c.base_low, (w & c.high) | c.base_high, (x & c.low) | c.base_low, (x & c.high) | c.base_high);
+}
+// z of a pair of scales, and what remains of their groups' values: low - 16 scale - z as (low + 8 scale) - (24 scale + z),
+// whose second part is exact.
+__device__ __forceinline__ uint32_t code_zero(uint32_t scale) { return pk_fma(scale, 0xce00ce00u, 0x80008000u); }
+__device__ __forceinline__ uint32_t middles(uint32_t low, uint32_t scale, uint32_t z) {
+  const uint32_t mid = pk_fma(scale, 0x48004800u, low), err = pk_fma(scale, 0x4e004e00u, z);
+  return pk_fma(err, 0xbc00bc00u, mid);
+}
+// a + b * (x of lane L of this lane's 16).
+template <int L>
+__device__ __forceinline__ float fma_row_lane(float x, float b, float a) {
+  return fmaf(__int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x150 + L, 0xf, 0xf, true)), b, a);
+}
+
+// The dwords of a key's row, ND consecutive ones per lane group as loaded, dealt out so that lane group g of word G holds one
+// of group G's four (dword 4 G + g; with two words in the order 0, 2, 1, 3).
+template <int ND>
+__device__ __forceinline__ void deal_words(uint32_t (&w)[ND]) {
+  auto swap32 = [](uint32_t& a, uint32_t& b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0], b = r[1];
+  };
+  auto swap16 = [](uint32_t& a, uint32_t& b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = r[0], b = r[1];
+  };
+  if constexpr (ND == 4) {
+    swap32(w[0], w[2]);
+    swap32(w[1], w[3]);
+    swap16(w[0], w[1]);
+    swap16(w[2], w[3]);
+  } else if constexpr (ND == 2) {
+    swap32(w[0], w[1]);
+  }
+}
+
+template <int N>
+struct Words {
+  uint32_t w[N];
+};
+template <int N>
+__device__ __forceinline__ Words<N> load_words(const char* p) {
+  Words<N> r;
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    r.w[0] = v.x, r.w[1] = v.y;
+  } else {
+    r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+  return r;
+}
+
+// What a wave holds of one step: two 16-key tiles.
+template <int ND>
+struct Step4 {
+  Words<ND> k[2];      // dwords ND g .. of key r
+  Words<ND> v[2];
+  uint32_t ks[2];      // (scale, low) of the lane's place in the row's [4 keys][ND]
+  uint32_t kr[2];      // (scale, low) of key r, group g
+  uint4 vm[2];         // scales and lows of quad g, the group of the lane's dims
+};
+
+struct Int4Divs {
+  DivU32 kv_heads, qtiles, group, tiles;
+};
+
+// The sum of x over the 4 lane groups (a permlane swap of a register with itself leaves a lane's own value in one result, its
+// partner's in the other).
+__device__ __forceinline__ float sum_groups(float x) {
+  const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r16[0]) + __uint_as_float(r16[1]);
+  const auto r32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r32[0]) + __uint_as_float(r32[1]);
+}
+__device__ __forceinline__ float max_groups(float x) {
+  const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = max_score(__uint_as_float(r16[0]), __uint_as_float(r16[1]));
+  const auto r32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return max_score(__uint_as_float(r32[0]), __uint_as_float(r32[1]));
+}
+
 template <int DT, int D>
-__global__ __launch_bounds__(D < 64 ? 64 : D) void merge_int4_kernel(Int4Attn p) {
+__global__ __launch_bounds__(64 * kAttnWaves, D == 128 ? 3 : 4) void attention_int4_mfma_kernel(Int4Attn p, Int4Divs dv) {
+  constexpr int WAVES = kAttnWaves;
+  constexpr int ND = D / 32;
+  constexpr int NB = D / 16;     // 16-row blocks of the result
+  constexpr int STEP = 2 * kTile;
+  constexpr int ACC = D + 4;     // floats of a query's accumulators in LDS
+  extern __shared__ __attribute__((aligned(16))) float s_mem[];  // [waves][queries] (max, sum), then [waves][queries][ACC]
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int g = lane >> 4, r = lane & 15;
+  const int rest = (int)udiv(blockIdx.x, dv.kv_heads);
+  const int kvh = (int)blockIdx.x - rest * p.kv_heads;
+  const int b = (int)udiv(rest, dv.qtiles);
+  const int qt = rest - b * (int)dv.qtiles.d;
+  const int chunk = blockIdx.y;
+  const int rows = p.group * p.qlen;       // queries of the KV head
+  const int count = min(16, rows - qt * 16);  // of this workgroup
+  const int last_q = (int)udiv(qt * 16 + count - 1, dv.group);
+  // The queries' loads go out first: vector loads return in order, and the keys' behind them are what takes long.
+  const int x = min(qt * 16 + r, rows - 1);
+  const int qi = (int)udiv(x, dv.group), h = kvh * p.group + x - qi * p.group;
+  uint4 q_raw[ND];
+  {
+    const char* q = p.q + (int64_t)b * p.qsb + (int64_t)qi * p.qsq + (int64_t)h * p.qsh;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)  // dims 32 i + 8 times deal_words' order of g
+      q_raw[i] = *reinterpret_cast<const uint4*>(q + 16 * (4 * i + (ND == 2 ? (g & 1) * 2 + (g >> 1) : g)));
+  }
+  const int lim = p.nb > 0 ? visible(p, b, last_q) : 0;  // keys any of its queries sees
+  const int t_begin = chunk * p.chunk, t_end = min(lim, t_begin + p.chunk);
+  if (t_begin >= lim && chunk > 0) return;
+  const int32_t* trow = p.tables + (int64_t)(p.trows ? scalar_word(p.trows + b) : b) * p.tstride;
+  const int last_tile = (t_end - 1) >> 4;
+
+  // The two tiles of a step. One behind a block id outside the pool reads block 0 instead and counts for nothing.
+  struct Tiles {
+    uint64_t at[2];
+    bool ok[2];
+  };
+  const uint64_t head_at = (uint64_t)kvh * p.tiles * (10 * D);
+  const uint32_t block_bytes = (uint32_t)(p.kv_heads * p.tiles * (10 * D));
+  auto find = [&](int t0) __attribute__((always_inline)) -> Tiles {
+    Tiles r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t tile = (uint32_t)min((t0 >> 4) + i, last_tile);
+      const uint32_t blk_i = udiv(tile, dv.tiles);
+      const uint32_t blk = (uint32_t)scalar_word(trow + blk_i);
+      r.ok[i] = blk < (uint32_t)p.nb;
+      r.at[i] = head_at + (uint64_t)(r.ok[i] ? blk : 0u) * block_bytes + (tile - blk_i * dv.tiles.d) * (10 * D);
+    }
+    return r;
+  };
+  using Step = Step4<ND>;
+  const uint32_t k_off = r * (D / 2) + g * (D / 8), kr_off = 8 * D + (r * ND + g * ND / 4) * 4;
+  const uint32_t ks_off = 8 * D + (g * 4 * ND + r % (4 * ND)) * 4;
+  const uint32_t v_off = g * 2 * D + r * (D / 8), vm_off = 8 * D + (g * ND + r * ND / 16) * 16;
+  Step cur;
+  auto load_k = [&](const Tiles& t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const char* k = p.k_pool + t.at[i];
+      cur.k[i] = load_words<ND>(k + k_off);
+      cur.ks[i] = *reinterpret_cast<const uint32_t*>(k + ks_off);
+      cur.kr[i] = *reinterpret_cast<const uint32_t*>(k + kr_off);
+    }
+  };
+  auto load_v = [&](const Tiles& t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const char* v = p.v_pool + t.at[i];
+      cur.v[i] = load_words<ND>(v + v_off);
+      cur.vm[i] = *reinterpret_cast<const uint4*>(v + vm_off);
+    }
+  };
+  // The registers of a step's K take the next step's as soon as they are read, and V's theirs: each load has the other
+  // half of a step to arrive in, and a third more waves are resident than with a second set (whose registers would not
+  // fit three waves per SIMD at D = 128: spills, which wait for every load ahead of them). Tiles are looked up two steps
+  // ahead; those past the end are the last tile again.
+  Tiles where{}, then{};
+  int t0 = t_begin + wave * STEP;
+  if (t0 < t_end) {
+    where = find(t0);
+    then = find(t0 + WAVES * STEP);
+    load_k(where);
+    load_v(where);
+  }
+
+  const int len0 = scalar_word(p.lens + b);
+  auto seen = [&](int q) __attribute__((always_inline)) {
+    return min(max(len0 - (p.causal ? p.qlen - 1 - q : 0), 0), p.max_ctx);
+  };
+  const int mine = min(seen(qi), t_end);   // keys of this chunk this lane's query sees end here
+  const int least = min(seen((int)udiv(qt * 16, dv.group)), t_end);
+  // Q^T: lane (query r, g) holds 8 dims of product G.
+  uint4 qf[ND], qs;
+  float c = fmaxf(fabsf(p.scale_log2), 1.17549435e-38f);  // positive, as the maximum is taken over unscaled scores
+  const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+  {
+    float f[ND][8], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      unpack16<DT>(q_raw[i], f[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max_score(top, fabsf(f[i][e]));
+    }
+    top = max_groups(top);
+    const int ex = top > 0.f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) : 0;
+    c = ldexpf(c, ex);
+    // Of the group whose (scale, low) the lane's kr holds: its sum of q, and of q times the codes' bases.
+    float sum = 0.f, based = 0.f;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      uint32_t w[4];
+      float part[2] = {0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = pack2<SKV_F16>(ldexpf(f[i][2 * e], -ex), ldexpf(f[i][2 * e + 1], -ex)) ^ flip;
+        part[e & 1] += lo16<SKV_F16>(w[e]) + hi16<SKV_F16>(w[e]);
+      }
+      qf[i] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) part[e] = sum_groups(part[e]);
+      if (g * ND / 4 == i) sum = part[0] + part[1], based = -1024.f * part[0] - 64.f * part[1];
+    }
+    sum *= ND / 4.f;  // 4 / ND lane groups hold one group
+    based *= ND / 4.f;
+    auto head = [](float v) { return lo16<SKV_F16>(pack2<SKV_F16>(v, 0.f)); };
+    const float s0 = head(sum), b0 = head(based), b1 = head(based - b0);
+    qs = make_uint4(pack2<SKV_F16>(s0, sum - s0), pack2<SKV_F16>(b0, b1), pack2<SKV_F16>(based - b0 - b1, 0.f), 0u);
+  }
+  uint32_t code_mask = kCodeMask, code_base = kCodeBase;
+  CodeRegs rows_c{0x000f000fu, 0x64006400u, 0x00f000f0u, 0x54005400u};
+  asm volatile("" : "+s"(code_mask), "+v"(code_base));
+  asm volatile("" : "+s"(rows_c.low), "+s"(rows_c.high), "+v"(rows_c.base_low), "+v"(rows_c.base_high));
+
+  float m = kNegInf, ref = 0.f;
+  f32x4 acc[NB], rest_acc = f32x4{0.f, 0.f, 0.f, 0.f};  // rows 4 g: the middles' part of the lane's group; 4 g + 1: the weights' sum
+#pragma unroll
+  for (int i = 0; i < NB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const bool sum_row = (r & 3) == 1;
+
+  while (t0 < t_end) {
+    const bool ok0 = where.ok[0], ok1 = where.ok[1];
+    const Tiles later = find(t0 + 2 * WAVES * STEP);
+    f32x4 s[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t low = __builtin_amdgcn_perm(cur.kr[i], cur.kr[i], 0x03020302u);
+      const uint32_t scale = __builtin_amdgcn_perm(cur.kr[i], cur.kr[i], 0x01000100u);
+      const float sf = lo16<SKV_F16>(cur.ks[i]);
+      s[i] = mfma_16x16x32<SKV_F16>(make_uint4(low, scale, scale, 0u), qs, f32x4{0.f, 0.f, 0.f, 0.f});
+      f32x4 t[ND];
+      deal_words<ND>(cur.k[i].w);
+#pragma unroll
+      for (int e = 0; e < ND; ++e) {
+        const uint32_t w = cur.k[i].w[e];
+        t[e] = mfma_16x16x32<SKV_F16>(code_row(w, rows_c), qf[e], f32x4{0.f, 0.f, 0.f, 0.f});
+      }
+      auto scaled = [&](auto e_c) __attribute__((always_inline)) {
+        constexpr int E = decltype(e_c)::value;
+        if constexpr (E < ND) {
+          s[i][0] = fma_row_lane<E>(sf, t[E][0], s[i][0]);
+          s[i][1] = fma_row_lane<ND + E>(sf, t[E][1], s[i][1]);
+          s[i][2] = fma_row_lane<2 * ND + E>(sf, t[E][2], s[i][2]);
+          s[i][3] = fma_row_lane<3 * ND + E>(sf, t[E][3], s[i][3]);
+        }
+      };
+      scaled(std::integral_constant<int, 0>{});
+      scaled(std::integral_constant<int, 1>{});
+      scaled(std::integral_constant<int, 2>{});
+      scaled(std::integral_constant<int, 3>{});
+    }
+    load_k(then);
+    __builtin_amdgcn_sched_barrier(0);
+    // A step with a key that some query does not see, or behind an invalid block id (wave-uniform).
+    if (t0 + STEP > least || !(ok0 && ok1)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        // What a slot past the row's end holds may be anything: those keys' scales and offsets become zeros, as do those
+        // of a tile behind an invalid block id.
+        const int base = t0 + kTile * i + 4 * g;
+        const int end = (i == 0 ? ok0 : ok1) ? t_end : 0;
+        const bool z0 = base >= end, z1 = base + 1 >= end, z2 = base + 2 >= end, z3 = base + 3 >= end;
+        const uint32_t m02 = (z0 ? 0u : 0xffffu) | (z2 ? 0u : 0xffff0000u), m13 = (z1 ? 0u : 0xffffu) | (z3 ? 0u : 0xffff0000u);
+        cur.vm[i].x &= m02, cur.vm[i].y &= m13, cur.vm[i].z &= m02, cur.vm[i].w &= m13;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][e] = base + e < min(mine, end) ? s[i][e] : kNegInf;
+      }
+    }
+    float mx = kNegInf;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx = max_score(mx, s[i][e]);
+    if (__builtin_amdgcn_ballot_w64(mx * c > m + kLazyMaxLog2) != 0) {  // wave-uniform
+      mx = max_groups(mx);
+      const float mn = max_score(m, mx * c);
+      ref = mn == kNegInf ? 0.f : mn;
+      const float alpha = __builtin_amdgcn_exp2f(m - ref);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) acc[i] *= alpha;
+      rest_acc *= alpha;
+      m = mn;
+    }
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[4 * i + e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], c, kWeightLog2 - ref));
+    uint32_t head[4], tail[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int k = 4 * (e >> 1) + (e & 1);  // keys 0, 2 and 1, 3 of each tile
+      head[e] = pack2<SKV_F16>(w[k], w[k + 2]);
+      tail[e] = pack2<SKV_F16>(fmaf(lo16<SKV_F16>(head[e]), -1.f, w[k]), fmaf(hi16<SKV_F16>(head[e]), -1.f, w[k + 2]));
+    }
+    const uint4 pt[2] = {make_uint4(head[0], head[1], head[2], head[3]), make_uint4(tail[0], tail[1], tail[2], tail[3])};
+    uint32_t z02[2], z13[2], mid[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      z02[i] = code_zero(cur.vm[i].x), z13[i] = code_zero(cur.vm[i].y);
+      mid[2 * i] = middles(cur.vm[i].z, cur.vm[i].x, z02[i]);
+      mid[2 * i + 1] = middles(cur.vm[i].w, cur.vm[i].y, z13[i]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mid[e] = sum_row ? 0x3c003c00u : mid[e];
+    const uint4 rest_a = make_uint4(mid[0], mid[1], mid[2], mid[3]);
+#pragma unroll
+    for (int o = 0; o < 2; ++o) rest_acc = mfma_16x16x32<SKV_F16>(rest_a, pt[o], rest_acc);
+#pragma unroll
+    for (int y = 0; y < ND; ++y) {
+      const uint32_t wa = cur.v[0].w[y], wb = cur.v[1].w[y];
+      const uint4 even = make_uint4(
+          pk_fma(code_pair<0>(wa, code_mask, code_base), cur.vm[0].x, z02[0]), pk_fma(code_pair<2>(wa, code_mask, code_base), cur.vm[0].y, z13[0]),
+          pk_fma(code_pair<0>(wb, code_mask, code_base), cur.vm[1].x, z02[1]), pk_fma(code_pair<2>(wb, code_mask, code_base), cur.vm[1].y, z13[1]));
+      const uint4 odd = make_uint4(
+          pk_fma(code_pair<1>(wa, code_mask, code_base), cur.vm[0].x, z02[0]), pk_fma(code_pair<3>(wa, code_mask, code_base), cur.vm[0].y, z13[0]),
+          pk_fma(code_pair<1>(wb, code_mask, code_base), cur.vm[1].x, z02[1]), pk_fma(code_pair<3>(wb, code_mask, code_base), cur.vm[1].y, z13[1]));
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        acc[2 * y] = mfma_16x16x32<SKV_F16>(even, pt[o], acc[2 * y]);
+        acc[2 * y + 1] = mfma_16x16x32<SKV_F16>(odd, pt[o], acc[2 * y + 1]);
+      }
+    }
+    load_v(then);
+    __builtin_amdgcn_sched_barrier(0);
+    t0 += WAVES * STEP;
+    where = then;
+    then = later;
+  }
+  const float l = rest_acc[1];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) acc[i] += rest_acc[0];
+  // Lane (g, query r) holds dims (4 g + i) D / 16 + block in acc[block][i].
+  float2* s_ml = reinterpret_cast<float2*>(s_mem);
+  float* s_acc = s_mem + 2 * WAVES * count;
+  if (r < count) {
+    if (g == 0) s_ml[wave * count + r] = make_float2(m, l);
+    float* a = s_acc + (wave * count + r) * ACC + g * (D / 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < NB; ++e) a[i * NB + e] = acc[e][i];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < count * (D / 2); i += 64 * WAVES) {
+    const int y = i / (D / 2), d = 2 * (i % (D / 2));
+    float mm = s_ml[y].x;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) mm = max_score(mm, s_ml[w * count + y].x);
+    const float base = mm == kNegInf ? 0.f : mm;
+    float sum = 0.f, a0 = 0.f, a1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float2 ml = s_ml[w * count + y];
+      const float f = __builtin_amdgcn_exp2f(ml.x - base);
+      const float2 v = *reinterpret_cast<const float2*>(s_acc + (w * count + y) * ACC + d);
+      sum = fmaf(ml.y, f, sum);
+      a0 = fmaf(v.x, f, a0);
+      a1 = fmaf(v.y, f, a1);
+    }
+    const int xq = qt * 16 + y, oq = (int)udiv(xq, dv.group), oh = kvh * p.group + xq - oq * p.group;
+    if (p.nchunk > 1 && seen(oq) > p.chunk) {
+      float* rec = p.part + ((((int64_t)b * p.qlen + oq) * p.heads + oh) * p.nchunk + chunk) * (D + kPad);
+      *reinterpret_cast<float2*>(rec + kPad + d) = make_float2(a0, a1);
+      if (d == 0) *reinterpret_cast<float2*>(rec) = make_float2(mm, sum);
+    } else if (chunk == 0) {  // its keys lie in the first chunk
+      const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+      *reinterpret_cast<uint32_t*>(p.o + (int64_t)b * p.osb + (int64_t)oq * p.osq + (int64_t)oh * p.osh + 2 * d) =
+          pack2<DT>(a0 * inv, a1 * inv);
+    }
+  }
+}
+
+// Rows of several chunks: one workgroup per (row, query, head) joins the chunks' partials, D / 4 lanes a partial, 1024 / D
+// partials at once.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void merge_int4_kernel(Int4Attn p) {
+  constexpr int LANES = D / 4, SETS = 256 / LANES;
+  __shared__ __attribute__((aligned(16))) float s_acc[SETS][D];
+  __shared__ float s_red[8];
   const int h = blockIdx.x % p.heads;
   const int rest = blockIdx.x / p.heads;
   const int qi = rest % p.qlen, b = rest / p.qlen;
   const int len = visible(p, b, qi);
   const int n = (len + p.chunk - 1) / p.chunk;
-  if (n <= 1 || threadIdx.x >= D) return;
-  const int d = threadIdx.x;
+  if (n <= 1) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float* rec = p.part + (((int64_t)b * p.qlen + qi) * p.heads + h) * p.nchunk * (D + kPad);
   float mm = kNegInf;
-  for (int c = 0; c < n; ++c) mm = max_score(mm, rec[c * (D + kPad)]);
+  for (int c = threadIdx.x; c < n; c += 256) mm = max_score(mm, rec[(int64_t)c * (D + kPad)]);
+  mm = max_score(mm, xor_lane<1>(mm));
+  mm = max_score(mm, xor_lane<2>(mm));
+  mm = max_score(mm, xor_lane<4>(mm));
+  mm = max_score(mm, xor_lane<8>(mm));
+  mm = max_score(mm, xor_lane<16>(mm));
+  mm = max_score(mm, xor_lane<32>(mm));
+  if (lane == 0) s_red[wave] = mm;
+  __syncthreads();
+  mm = max_score(max_score(s_red[0], s_red[1]), max_score(s_red[2], s_red[3]));
   const float ref = mm == kNegInf ? 0.f : mm;
-  float l = 0.f, acc = 0.f;
-  for (int c = 0; c < n; ++c) {
-    const float f = __builtin_amdgcn_exp2f(rec[c * (D + kPad)] - ref);
-    l = fmaf(rec[c * (D + kPad) + 1], f, l);
-    acc = fmaf(rec[c * (D + kPad) + kPad + d], f, acc);
+  const int set = threadIdx.x / LANES, d = (threadIdx.x % LANES) * 4;
+  float l = 0.f;
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int c = set; c < n; c += SETS) {
+    const float* r = rec + (int64_t)c * (D + kPad);
+    const float f = __builtin_amdgcn_exp2f(r[0] - ref);
+    l = fmaf(r[1], f, l);
+    acc += f * *reinterpret_cast<const f32x4*>(r + kPad + d);
   }
-  const float out = l > 0.f || l != l ? acc / l : 0.f;
+  *reinterpret_cast<f32x4*>(&s_acc[set][d]) = acc;
+  // Each set's sum once: its lanes hold the same.
+  __shared__ float s_sum[SETS];
+  if (d == 0) s_sum[set] = l;
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  float out = 0.f, sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < SETS; ++i) {
+    out += s_acc[i][threadIdx.x];
+    sum += s_sum[i];
+  }
+  out = sum > 0.f || sum != sum ? out / sum : 0.f;
   char* o = p.o + (int64_t)b * p.osb + (int64_t)qi * p.osq + (int64_t)h * p.osh;
   if constexpr (DT == SKV_F32)
-    reinterpret_cast<float*>(o)[d] = out;
+    reinterpret_cast<float*>(o)[threadIdx.x] = out;
   else
-    reinterpret_cast<uint16_t*>(o)[d] = (uint16_t)pack2<DT>(out, 0.f);
+    reinterpret_cast<uint16_t*>(o)[threadIdx.x] = (uint16_t)pack2<DT>(out, 0.f);
 }
 
 // ---------------------------------------------------------------------------
@@ -442,20 +894,35 @@ __global__ __launch_bounds__(D < 64 ? 64 : D) void merge_int4_kernel(Int4Attn p)
 // ---------------------------------------------------------------------------
 constexpr int kChunkUnit = 64;  // chunks are multiples of this many keys
 
-int32_t pick_chunk4(int64_t rows, int32_t heads, int32_t max_ctx) {
+// Workgroups a call has before its keys are split.
+int64_t attn4_items(int32_t batch, int32_t q_len, int32_t heads, int32_t kv_heads, int32_t dtype) {
+  if (dtype == SKV_F32) return (int64_t)batch * q_len * heads;
+  return (int64_t)batch * cdiv((int64_t)(heads / kv_heads) * q_len, 16) * kv_heads;
+}
+
+// Key chunk of a call of `items` workgroups before its keys are split.
+int32_t pick_chunk4(int64_t items, int32_t d, int32_t max_ctx) {
   const int64_t units = cdiv(max_ctx > 0 ? max_ctx : 1, kChunkUnit);
-  const int64_t items = rows * heads;
-  int64_t chunks = items >= 1024 ? 1 : cdiv(1024, items > 0 ? items : 1);
-  const int64_t most = cdiv(units, 4);
-  chunks = chunks > most ? most : chunks;
+  int64_t chunks = max_ctx <= 512 || items >= (d == 128 ? 512 : 1024) ? 1 : 1024 / (items > 0 ? items : 1);
+  const int64_t most = cdiv(units, 2);
+  chunks = chunks > most ? most : (chunks < 1 ? 1 : chunks);
   return (int32_t)(cdiv(units, chunks) * kChunkUnit);
 }
 
 template <int DT, int D>
 void launch_attn4(const Int4Attn& p, hipStream_t stream) {
   const uint32_t items = (uint32_t)((int64_t)p.batch * p.qlen * p.heads);
-  hipLaunchKernelGGL((attention_int4_kernel<DT, D>), dim3(items, p.nchunk), dim3(64 * kAttnWaves), 0, stream, p);
-  if (p.nchunk > 1) hipLaunchKernelGGL((merge_int4_kernel<DT, D>), dim3(items), dim3(D < 64 ? 64 : D), 0, stream, p);
+  if constexpr (DT != SKV_F32) {
+    const int rows = p.group * p.qlen, qtiles = (rows + 15) / 16;
+    const uint32_t lds = (uint32_t)(kAttnWaves * (rows < 16 ? rows : 16) * (2 + D + 4) * sizeof(float));
+    const Int4Divs dv{make_div((uint32_t)p.kv_heads), make_div((uint32_t)qtiles), make_div((uint32_t)p.group),
+                      make_div((uint32_t)p.tiles)};
+    hipLaunchKernelGGL((attention_int4_mfma_kernel<DT, D>), dim3((uint32_t)(p.batch * qtiles * p.kv_heads), p.nchunk),
+                       dim3(64 * kAttnWaves), lds, stream, p, dv);
+  } else {
+    hipLaunchKernelGGL((attention_int4_kernel<DT, D>), dim3(items, p.nchunk), dim3(64 * kAttnWaves), 0, stream, p);
+  }
+  if (p.nchunk > 1) hipLaunchKernelGGL((merge_int4_kernel<DT, D>), dim3(items), dim3(256), 0, stream, p);
 }
 template <int DT>
 void launch_attn4_d(int d, const Int4Attn& p, hipStream_t stream) {
@@ -625,8 +1092,8 @@ int skv_gather_int4(const void* k_pool, const void* v_pool, const int32_t* block
 
 int32_t skv_int4_chunk_tokens(int32_t batch, int32_t q_len, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                               int32_t max_ctx, int32_t dtype) {
-  if (batch <= 0 || q_len <= 0 || num_heads <= 0) return kChunkUnit;
-  return pick_chunk4((int64_t)batch * q_len, num_heads, max_ctx);
+  if (batch <= 0 || q_len <= 0 || num_heads <= 0 || num_kv_heads <= 0) return kChunkUnit;
+  return pick_chunk4(attn4_items(batch, q_len, num_heads, num_kv_heads, dtype), head_dim, max_ctx);
 }
 
 int64_t skv_int4_workspace_bytes(int32_t batch, int32_t q_len, int32_t num_heads, int32_t head_dim, int32_t max_ctx,
