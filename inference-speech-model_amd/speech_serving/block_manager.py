@@ -12,6 +12,10 @@ allocation [num_layers, 2, num_blocks, block_size, num_kv_heads, head_dim], so
 a token row of one layer (num_kv_heads * head_dim elements) is contiguous and
 every block is block_size such rows back to back. The decode kernels read
 these pools directly through per-request block tables.
+
+With kv_bits=4 the pools are uint8 tensors of the 4-bit cache (native.int4_pool_shape),
+[num_layers, 2, num_blocks, num_kv_heads, block_size / 16, 10 * head_dim] in one allocation:
+native.append_int4 writes key_pool[l] / value_pool[l], native.paged_attention_int4 reads them.
 """
 from __future__ import annotations
 
@@ -36,6 +40,7 @@ class BlockManager:
         num_blocks: Optional[int] = None,
         dtype: torch.dtype = torch.float16,
         device: str = "cuda",
+        kv_bits: Optional[int] = None,
     ):
         for name, val in (("num_layers", num_layers), ("num_kv_heads", num_kv_heads), ("head_dim", head_dim),
                           ("block_size", block_size)):
@@ -47,8 +52,14 @@ class BlockManager:
         self.num_kv_heads = num_kv_heads
         self.head_dim = head_dim
         self.block_size = block_size
+        if kv_bits not in (None, 4):
+            raise ValueError(f"kv_bits must be None (the dtype's own) or 4, got {kv_bits}")
+        if kv_bits == 4 and (block_size % 16 or head_dim not in (32, 64, 128)):
+            raise ValueError(f"a 4-bit cache takes blocks of a multiple of 16 tokens and head_dim 32, 64 or 128, "
+                             f"got {block_size} and {head_dim}")
         self.dtype = dtype
         self.device = device
+        self.kv_bits = kv_bits
 
         if num_blocks is None:
             num_blocks = self._auto_num_blocks()
@@ -56,8 +67,11 @@ class BlockManager:
             raise ValueError(f"num_blocks must be > 0, got {num_blocks}")
         self.num_blocks = num_blocks
 
-        self.arena = torch.zeros((num_layers, 2, num_blocks, block_size, num_kv_heads, head_dim), dtype=dtype,
-                                 device=device)
+        if kv_bits == 4:
+            pool, pool_dtype = (num_blocks, num_kv_heads, block_size // 16, 10 * head_dim), torch.uint8
+        else:
+            pool, pool_dtype = (num_blocks, block_size, num_kv_heads, head_dim), dtype
+        self.arena = torch.zeros((num_layers, 2, *pool), dtype=pool_dtype, device=device)
         self.key_pool: List[torch.Tensor] = [self.arena[l, 0] for l in range(num_layers)]
         self.value_pool: List[torch.Tensor] = [self.arena[l, 1] for l in range(num_layers)]
 
@@ -68,6 +82,8 @@ class BlockManager:
     # ------------------------------------------------------------------ sizing
     def block_bytes(self) -> int:
         """Bytes of one block across all layers, K and V."""
+        if self.kv_bits == 4:  # 5 bits an element: codes, and two fp16 per 32
+            return self.num_layers * 2 * self.block_size * self.num_kv_heads * self.head_dim * 5 // 8
         return (self.num_layers * 2 * self.block_size * self.num_kv_heads * self.head_dim
                 * _element_size(self.dtype))
 
@@ -112,9 +128,11 @@ class BlockManager:
         return (num_tokens + self.block_size - 1) // self.block_size
 
     def gather(self, layer: int, block_tables: torch.Tensor, lens: torch.Tensor, max_len: int):
-        """Contiguous zero-padded [B, H, max_len, D] K and V of `layer` (HIP gather kernel)."""
+        """Contiguous zero-padded [B, H, max_len, D] K and V of `layer` (HIP gather kernel), in `dtype`."""
         from . import native
 
+        if self.kv_bits == 4:
+            return native.gather_int4(self.key_pool[layer], self.value_pool[layer], block_tables, lens, max_len, self.dtype)
         return native.gather(self.key_pool[layer], self.value_pool[layer], block_tables, lens, max_len)
 
     # ------------------------------------------------------------------ telemetry

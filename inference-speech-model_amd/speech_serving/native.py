@@ -1068,7 +1068,7 @@ def _rows3(what: str, t: torch.Tensor, name: str, shape: Tuple[int, int, int], d
             ok = (sn if n > 1 else sh) >= d
         if not ok:
             raise RuntimeError(f"{what}: {name} must have a contiguous last dim, 16-byte aligned rows and no overlap")
-    return t if ok else t.contiguous()
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def rotary_table(max_positions: int, rot_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -1254,7 +1254,7 @@ def paged_attention_int4(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     code = _code(q.dtype)
     epl = 16 // q.element_size()
     if q4.stride(3) != 1 or q4.data_ptr() % 16 or any(st % epl for st in q4.stride()[:3]):
-        q4 = q4.contiguous()
+        q4 = q4.clone(memory_format=torch.contiguous_format)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     o4 = _q4(out, "out")
