@@ -523,7 +523,7 @@ SKV_API int skv_paged_attention_int4(const void* q, int64_t q_stride_b, int64_t 
  *   q, out [N, num_heads, D], k, v [N, num_kv_heads, D] rows at their own strides (slices of a fused projection are fine);
  *   sequence s is rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (int32 [num_seqs + 1] device, non-decreasing, within
  *   0..N), of any length, 0 included; its query i sees its keys 0..i, whatever the later keys hold. Rows of out that belong
- *   to no sequence are left as they are. head_dim in {16, 32, 64, 128}.
+ *   to no sequence are left as they are. head_dim in {16, 32, 64, 128}; row strides of k and v from 0 to below 16 MiB.
  * Replaces, for prompts of different lengths, the padded batch of models.py:126-165.
  */
 SKV_API int skv_prompt_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h, const void* k, int64_t k_stride_n,

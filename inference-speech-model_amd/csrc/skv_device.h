@@ -162,6 +162,18 @@ template <> __device__ __forceinline__ void unpack16<SKV_BF16>(const uint4& v, f
   }
 }
 
+// N consecutive floats, 16-byte aligned.
+template <int N>
+__device__ __forceinline__ void load_floats(const float* p, float* f) {
+  static_assert(N % 4 == 0, "load_floats: whole 16-byte vectors");
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p + i);
+    f[i] = __uint_as_float(v.x), f[i + 1] = __uint_as_float(v.y);
+    f[i + 2] = __uint_as_float(v.z), f[i + 3] = __uint_as_float(v.w);
+  }
+}
+
 // Sum over the EPL lane elements of q*k in fp32. fp16/bf16 use the packed
 // v_dot2_f32_{f16,bf16} (products of 16-bit values are exact in fp32).
 template <int DT> __device__ __forceinline__ float dot16(const uint4& q, const uint4& k);

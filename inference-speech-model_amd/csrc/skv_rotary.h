@@ -29,15 +29,4 @@ __device__ __forceinline__ void rotate_pair(float& a, float& b, float c, float s
   b = bc + as;
 }
 
-template <int N>
-__device__ __forceinline__ void load_floats(const float* p, float* f) {
-  static_assert(N % 4 == 0, "load_floats: whole 16-byte vectors");
-#pragma unroll
-  for (int i = 0; i < N; i += 4) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p + i);
-    f[i] = __uint_as_float(v.x), f[i + 1] = __uint_as_float(v.y);
-    f[i + 2] = __uint_as_float(v.z), f[i + 3] = __uint_as_float(v.w);
-  }
-}
-
 }  // namespace skv

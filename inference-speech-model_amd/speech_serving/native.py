@@ -1025,41 +1025,38 @@ INT4_HEAD_DIMS = (32, 64, 128)
 INT4_TILE = 16  # tokens of a tile (kTile of the library)
 
 
-def _one_device(what: str, *named: Tuple[str, Optional[torch.Tensor]]) -> int:
+def _one_device(what: str, *tensors: Optional[torch.Tensor]) -> int:
     """The GPU that all the given tensors are on; RuntimeError when they are not on one."""
-    dev = -1
-    for name, t in named:
-        if t is None:
-            continue
-        idx = t.get_device()
-        if idx < 0:
-            _gpu(t, name)
-        if dev < 0:
-            dev = idx
-        elif idx != dev:
-            raise RuntimeError(f"{what}: {name} is on GPU {idx}, the other tensors on GPU {dev}")
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != dev or dev < 0):
+            raise RuntimeError(f"{what}: all tensors must be on one GPU (got devices "
+                               f"{[str(x.device) for x in tensors if x is not None]}); the HIP kernels have no CPU path")
     return dev
+
+
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _call(what: str, dev: int, *args) -> None:
     """One library call on the current stream of GPU `dev`, which is made the current device for it."""
-    fn = getattr(lib(), what)
-    if dev == torch.cuda.current_device():
-        _check(fn(*args, _stream(torch.device("cuda", dev))), what)
+    fn = getattr(_lib or lib(), what)
+    if dev == _get_device():
+        rc = fn(*args, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream)
     else:
         with torch.cuda.device(dev):
-            _check(fn(*args, _stream(torch.device("cuda", dev))), what)
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _check(rc, what)
 
 
-def _rows3(what: str, t: torch.Tensor, name: str, shape: Tuple[int, int, int], dtype: torch.dtype,
-           written: bool = False) -> torch.Tensor:
-    """t as [N, H, D] rows with contiguous, 16-byte aligned vectors: a copy where an input is laid out otherwise, RuntimeError
-    where an output is (or where its rows overlap)."""
-    if tuple(t.shape) != shape or t.dtype != dtype:
+def _rows3(what: str, t: torch.Tensor, name: str, shape, dtype: torch.dtype, written: bool = False):
+    """(t, row stride, head stride) of t as [N, H, D] rows with contiguous, 16-byte aligned vectors: a copy where an input is
+    laid out otherwise, RuntimeError where an output is (or where its rows overlap)."""
+    if t.shape != shape or t.dtype != dtype:
         raise RuntimeError(f"{what}: {name} must be {list(shape)} {dtype}, got {list(t.shape)} {t.dtype}")
-    epl = 16 // t.element_size()
     sn, sh, sd = t.stride()
-    ok = (sd == 1 or shape[2] == 1) and sn % epl == 0 and sh % epl == 0 and t.data_ptr() % 16 == 0
+    ok = (sd == 1 or shape[2] == 1) and not (sn | sh) & (3 if dtype is torch.float32 else 7) and not t.data_ptr() & 15
     if written:
         n, h, d = shape
         if ok and n > 1 and h > 1:
@@ -1068,7 +1065,10 @@ def _rows3(what: str, t: torch.Tensor, name: str, shape: Tuple[int, int, int], d
             ok = (sn if n > 1 else sh) >= d
         if not ok:
             raise RuntimeError(f"{what}: {name} must have a contiguous last dim, 16-byte aligned rows and no overlap")
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    if ok:
+        return t, sn, sh
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride(0), t.stride(1)
 
 
 def rotary_table(max_positions: int, rot_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -1087,42 +1087,52 @@ def _index64(what: str, t: torch.Tensor, name: str, n: int) -> torch.Tensor:
     return t.contiguous()
 
 
-def _append_rows(what: str, k_new, v_new, slot_mapping, positions, cos_sin, q, q_out, k_out):
-    """(device, the argument list of a rotating append up to its pools, q_out, what keeps the arguments alive)."""
+def _append_rows(what: str, k_new, v_new, k_pool, v_pool, slot_mapping, positions, cos_sin, q, q_out, k_out):
+    """(device, dtype code, the arguments of a rotating append up to its sizes, q_out, what keeps the arguments alive)."""
     if k_new.dim() != 3:
         raise RuntimeError(f"{what}: k_new must be [N, H, D], got {list(k_new.shape)}")
-    dev = _one_device(what, ("k_new", k_new), ("v_new", v_new), ("slot_mapping", slot_mapping), ("positions", positions),
-                      ("cos_sin", cos_sin), ("q", q), ("q_out", q_out), ("k_out", k_out))
-    n, h, d = k_new.shape
+    dev = _one_device(what, k_new, v_new, k_pool, v_pool, slot_mapping, positions, cos_sin, q, q_out, k_out)
+    shape = k_new.shape
+    n = shape[0]
     dt = k_new.dtype
-    _code(dt)
-    k_new = _rows3(what, k_new, "k_new", (n, h, d), dt)
-    v_new = _rows3(what, v_new, "v_new", (n, h, d), dt)
+    code = _code(dt)
+    k_new, kn, kh = _rows3(what, k_new, "k_new", shape, dt)
+    v_new, vn, vh = _rows3(what, v_new, "v_new", shape, dt)
     slot_mapping = _index64(what, slot_mapping, "slot_mapping", n)
-    if (cos_sin is None) != (positions is None):
-        raise RuntimeError(f"{what}: positions and cos_sin go together")
-    if cos_sin is None and (q is not None or k_out is not None):
-        raise RuntimeError(f"{what}: q and k_out come with positions and cos_sin")
-    if q is None and q_out is not None:
-        raise RuntimeError(f"{what}: q_out comes with q")
-    if cos_sin is not None:
+    q_args = qo_args = ko_args = (None, 0, 0)
+    rotary = (None, None, 0, 0)
+    if cos_sin is None:
+        if positions is not None or q is not None or k_out is not None:
+            raise RuntimeError(f"{what}: positions, q and k_out come with cos_sin")
+    else:
+        if positions is None:
+            raise RuntimeError(f"{what}: cos_sin comes with positions")
         positions = _index64(what, positions, "positions", n)
         if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous():
             raise RuntimeError(f"{what}: cos_sin must be contiguous float32 [positions, rot_dim]")
-    args = []
+        rotary = (positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[1])
+    heads = 0
     if q is not None:
         if q.dim() != 3:
             raise RuntimeError(f"{what}: q must be [N, heads, D], got {list(q.shape)}")
-        q = _rows3(what, q, "q", (n, q.shape[1], d), dt)
+        heads = q.shape[1]
+        q_shape = (n, heads, shape[2])
+        q, qn, qh = _rows3(what, q, "q", q_shape, dt)
+        q_args = (q.data_ptr(), qn, qh)
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=dt, device=q.device)
+            q_out = torch.empty(q_shape, dtype=dt, device=q.device)
+            qo_args = (q_out.data_ptr(), heads * shape[2], shape[2])
         else:
-            q_out = _rows3(what, q_out, "q_out", tuple(q.shape), dt, written=True)
+            _, qn, qh = _rows3(what, q_out, "q_out", q_shape, dt, written=True)
+            qo_args = (q_out.data_ptr(), qn, qh)
+    elif q_out is not None:
+        raise RuntimeError(f"{what}: q_out comes with q")
     if k_out is not None:
-        k_out = _rows3(what, k_out, "k_out", (n, h, d), dt, written=True)
-    for t in (q, k_new, v_new, q_out, k_out):
-        args += [None, 0, 0] if t is None else [t.data_ptr(), t.stride(0), t.stride(1)]
-    return dev, args, q_out, (q, k_new, v_new, slot_mapping, positions)
+        _, kon, koh = _rows3(what, k_out, "k_out", shape, dt, written=True)
+        ko_args = (k_out.data_ptr(), kon, koh)
+    args = (*q_args, k_new.data_ptr(), kn, kh, v_new.data_ptr(), vn, vh, *qo_args, *ko_args, k_pool.data_ptr(),
+            v_pool.data_ptr(), slot_mapping.data_ptr(), *rotary)
+    return dev, code, heads, args, q_out, (q, k_new, v_new, slot_mapping, positions)
 
 
 def append_rotary(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -1140,16 +1150,14 @@ def append_rotary(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor
     what = "append_rotary"
     if cos_sin is None or positions is None:
         raise RuntimeError(f"{what}: positions and cos_sin are required (append() stores rows as they are)")
-    dev, args, q_out, keep = _append_rows(what, k_new, v_new, slot_mapping, positions, cos_sin, q, q_out, k_out)
+    dev, code, heads, args, q_out, keep = _append_rows(what, k_new, v_new, k_pool, v_pool, slot_mapping, positions, cos_sin, q,
+                                                       q_out, k_out)
     n, h, d = k_new.shape
     for t, name in ((k_pool, "k_pool"), (v_pool, "v_pool")):
-        if t.dim() != 4 or t.shape[2:] != (h, d) or t.shape != k_pool.shape or t.dtype != k_new.dtype or \
-                not t.is_contiguous() or t.get_device() != dev:
-            raise RuntimeError(f"{what}: {name} must be contiguous [num_blocks, block_size, {h}, {d}] {k_new.dtype} on the "
-                               f"rows' GPU, got {list(t.shape)} {t.dtype}")
-    _call("skv_append_rotary", dev, *args, k_pool.data_ptr(), v_pool.data_ptr(), keep[3].data_ptr(), keep[4].data_ptr(),
-          cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[1], 1 if interleaved else 0, n,
-          0 if q is None else q.shape[1], h, d, k_pool.shape[0] * k_pool.shape[1], _code(k_new.dtype))
+        if t.dim() != 4 or t.shape[2:] != (h, d) or t.shape != k_pool.shape or t.dtype != k_new.dtype or not t.is_contiguous():
+            raise RuntimeError(f"{what}: {name} must be contiguous [num_blocks, block_size, {h}, {d}] {k_new.dtype}, got "
+                               f"{list(t.shape)} {t.dtype}")
+    _call("skv_append_rotary", dev, *args, 1 if interleaved else 0, n, heads, h, d, k_pool.shape[0] * k_pool.shape[1], code)
     return q_out
 
 
@@ -1180,14 +1188,13 @@ def append_int4(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor, 
     least and greatest value. With positions and cos_sin the keys (and q, whose rotated rows are returned) are rotated first,
     as append_rotary does; the codes are those of the rotated row rounded to the rows' type."""
     what = "append_int4"
-    dev, args, q_out, keep = _append_rows(what, k_new, v_new, slot_mapping, positions, cos_sin, q, q_out, k_out)
     nb, bs, hp, dp = _int4_pools(what, k_pool, v_pool)
+    dev, code, heads, args, q_out, keep = _append_rows(what, k_new, v_new, k_pool, v_pool, slot_mapping, positions, cos_sin, q,
+                                                       q_out, k_out)
     n, h, d = k_new.shape
-    if (hp, dp) != (h, d) or k_pool.get_device() != dev or v_pool.get_device() != dev:
-        raise RuntimeError(f"{what}: pools of {hp} heads x {dp} do not fit rows [*, {h}, {d}], or are on another GPU")
-    _call("skv_append_int4", dev, *args, k_pool.data_ptr(), v_pool.data_ptr(), keep[3].data_ptr(), _ptr(keep[4]),
-          _ptr(cos_sin), 0 if cos_sin is None else cos_sin.shape[0], 0 if cos_sin is None else cos_sin.shape[1],
-          1 if interleaved else 0, n, 0 if q is None else q.shape[1], h, d, bs, nb, _code(k_new.dtype))
+    if (hp, dp) != (h, d):
+        raise RuntimeError(f"{what}: pools of {hp} heads x {dp} do not fit rows [*, {h}, {d}]")
+    _call("skv_append_int4", dev, *args, 1 if interleaved else 0, n, heads, h, d, bs, nb, code)
     return q_out
 
 
@@ -1197,8 +1204,7 @@ def gather_int4(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.
     """gather() from 4-bit pools: the values they hold as contiguous [B, H, max_len, D] of dtype, zero beyond lens[b]."""
     what = "gather_int4"
     block_tables, lens = _i32(block_tables, "block_tables"), _i32(lens, "lens")
-    dev = _one_device(what, ("k_pool", k_pool), ("v_pool", v_pool), ("block_tables", block_tables), ("lens", lens),
-                      ("k_out", k_out), ("v_out", v_out))
+    dev = _one_device(what, k_pool, v_pool, block_tables, lens, k_out, v_out)
     nb, bs, h, d = _int4_pools(what, k_pool, v_pool)
     if block_tables.dim() != 2 or lens.numel() < block_tables.shape[0]:
         raise RuntimeError(f"{what}: block_tables must be [B, max_blocks] and lens must cover the rows")
@@ -1238,8 +1244,7 @@ def paged_attention_int4(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     block_tables, ctx_lens = _i32(block_tables, "block_tables"), _i32(ctx_lens, "ctx_lens")
     if table_rows is not None:
         table_rows = _i32(table_rows, "table_rows")
-    dev = _one_device(what, ("q", q), ("k_pool", k_pool), ("v_pool", v_pool), ("block_tables", block_tables),
-                      ("ctx_lens", ctx_lens), ("table_rows", table_rows), ("out", out))
+    dev = _one_device(what, q, k_pool, v_pool, block_tables, ctx_lens, table_rows, out)
     nb, bs, hkv, dk = _int4_pools(what, k_pool, v_pool)
     q4 = _q4(q, "q")
     bsz, qlen, heads, d = q4.shape
@@ -1252,21 +1257,23 @@ def paged_attention_int4(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     if table_rows is not None and table_rows.numel() < bsz:
         raise RuntimeError(f"{what}: table_rows must cover the batch")
     code = _code(q.dtype)
-    epl = 16 // q.element_size()
-    if q4.stride(3) != 1 or q4.data_ptr() % 16 or any(st % epl for st in q4.stride()[:3]):
+    wide = 3 if q.dtype is torch.float32 else 7
+    qb, qq, qh, qd = q4.stride()
+    if qd != 1 or (qb | qq | qh) & wide or q4.data_ptr() & 15:
         q4 = q4.clone(memory_format=torch.contiguous_format)
+        qb, qq, qh, _ = q4.stride()
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     o4 = _q4(out, "out")
-    if tuple(o4.shape) != tuple(q4.shape) or o4.stride(3) != 1 or out.dtype != q.dtype:
+    ob, oq, oh, od = o4.stride()
+    if o4.shape != q4.shape or od != 1 or out.dtype != q.dtype:
         raise RuntimeError(f"{what}: out must match q's shape and type with contiguous head_dim")
     max_ctx = max(0, min(int(max_ctx), block_tables.shape[1] * bs))
     chunk, need = _int4_plan(bsz, qlen, heads, hkv, d, max_ctx, code, int(chunk_tokens))
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _call("skv_paged_attention_int4", dev, q4.data_ptr(), q4.stride(0), q4.stride(1), q4.stride(2), k_pool.data_ptr(),
-          v_pool.data_ptr(), block_tables.data_ptr(), block_tables.shape[1], _ptr(table_rows), ctx_lens.data_ptr(),
-          o4.data_ptr(), o4.stride(0), o4.stride(1), o4.stride(2), bsz, qlen, heads, hkv, d, bs, nb, max_ctx, float(scale),
-          SKV_ATTN_CAUSAL if causal else 0, code, chunk, _ptr(ws), need)
+    _call("skv_paged_attention_int4", dev, q4.data_ptr(), qb, qq, qh, k_pool.data_ptr(), v_pool.data_ptr(),
+          block_tables.data_ptr(), block_tables.shape[1], _ptr(table_rows), ctx_lens.data_ptr(), o4.data_ptr(), ob, oq, oh, bsz,
+          qlen, heads, hkv, d, bs, nb, max_ctx, scale, SKV_ATTN_CAUSAL if causal else 0, code, chunk, _ptr(ws), need)
     return out
 
 
@@ -1280,22 +1287,23 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     Reference math: speech_serving/models.py:126-165, per prompt."""
     what = "prompt_attention"
     cu_seqlens = _i32(cu_seqlens, "cu_seqlens")
-    dev = _one_device(what, ("q", q), ("k", k), ("v", v), ("cu_seqlens", cu_seqlens), ("out", out))
+    dev = _one_device(what, q, k, v, cu_seqlens, out)
     if q.dim() != 3 or k.dim() != 3:
         raise RuntimeError(f"{what}: q, k, v must be [N, heads, D], got {list(q.shape)}, {list(k.shape)}")
     n, heads, d = q.shape
     hkv = k.shape[1]
     if cu_seqlens.numel() < 1 or hkv == 0 or heads % hkv:
         raise RuntimeError(f"{what}: cu_seqlens must hold at least one entry, {heads} heads must be a multiple of {hkv}")
-    code = _code(q.dtype)
-    q = _rows3(what, q, "q", (n, heads, d), q.dtype)
-    k = _rows3(what, k, "k", (n, hkv, d), q.dtype)
-    v = _rows3(what, v, "v", (n, hkv, d), q.dtype)
+    dt = q.dtype
+    code = _code(dt)
+    q, qn, qh = _rows3(what, q, "q", (n, heads, d), dt)
+    k, kn, kh = _rows3(what, k, "k", (n, hkv, d), dt)
+    v, vn, vh = _rows3(what, v, "v", (n, hkv, d), dt)
     if out is None:
-        out = torch.empty((n, heads, d), dtype=q.dtype, device=q.device)
+        out = torch.empty((n, heads, d), dtype=dt, device=q.device)
+        on, oh = heads * d, d
     else:
-        _rows3(what, out, "out", (n, heads, d), q.dtype, written=True)
-    _call("skv_prompt_attention", dev, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-          v.data_ptr(), v.stride(0), v.stride(1), cu_seqlens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), n,
-          cu_seqlens.numel() - 1, heads, hkv, d, float(scale), code)
+        _, on, oh = _rows3(what, out, "out", (n, heads, d), dt, written=True)
+    _call("skv_prompt_attention", dev, q.data_ptr(), qn, qh, k.data_ptr(), kn, kh, v.data_ptr(), vn, vh,
+          cu_seqlens.data_ptr(), out.data_ptr(), on, oh, n, cu_seqlens.numel() - 1, heads, hkv, d, scale, code)
     return out

@@ -92,7 +92,8 @@ PROMPT = dict(q=P, qn=512, qh=64, k=P, kn=256, kh=64, v=P, vn=256, vh=64, cu=P, 
     (dict(dtype=5), EDTYPE, b"dtype"), (dict(d=48), EINVAL, b"head_dim"), (dict(d=256), EINVAL, b"head_dim"),
     (dict(n=-1), EINVAL, b"sizes"), (dict(seqs=-1), EINVAL, b"sizes"), (dict(heads=6), EINVAL, b"sizes"),
     (dict(kv=0), EINVAL, b"sizes"), (dict(q=None), EINVAL, b"null"), (dict(cu=None), EINVAL, b"null"),
-    (dict(o=P + 4), EALIGN, b"align"), (dict(vn=252), EALIGN, b"stride")])
+    (dict(o=P + 4), EALIGN, b"align"), (dict(vn=252), EALIGN, b"stride"), (dict(kn=-256), EINVAL, b"stride"),
+    (dict(vn=1 << 23), EINVAL, b"stride"), (dict(n=1 << 30), EINVAL, b"too large"), (dict(seqs=1 << 22), EINVAL, b"too large")])
 def test_prompt_attention_entry(lib, change, code, word):
     rc = lib.skv_prompt_attention(*{**PROMPT, **change}.values(), None)
     assert rc == code and word in lib.skv_last_error(), lib.skv_last_error()
