@@ -36,14 +36,15 @@ __device__ __forceinline__ uint32_t to_half_bits(float f) { return __builtin_bit
 // Append.
 // ---------------------------------------------------------------------------
 struct Int4Append {
-  Rows q, k, v, qo, ko;
+  Rows k, v, ko;
   char *k_pool, *v_pool;
   const int64_t* slots;
   int64_t num_slots;
   Rotary r;
-  DivU32 per_tok;  // lanes per token
-  uint32_t total;
-  int32_t q_heads, kv_heads;
+  DivU32 per_quad;  // lanes of 4 tokens
+  uint32_t total, n;
+  int32_t kv_heads;
+  uint32_t blocks;  // workgroups of K and V; the others rotate q
   DivU32 tiles;     // tiles per (block, head)
 };
 
@@ -75,106 +76,171 @@ __device__ __forceinline__ void round8(float* f) {
   }
 }
 
-// One lane per 8 dims of a row, D / 8 lanes (4 to 16, never across a wave) per row: K rows, V rows, then q rows, which are
-// only rotated. A rotated row's lanes all load before any stores, so q and k may be rotated in place. The codes are taken
-// from the rotated values rounded to the rows' type, what a 16-bit cache would hold.
+template <int OFF> __device__ __forceinline__ uint32_t xor_bits(uint32_t x) {
+  return __float_as_uint(xor_lane<OFF>(__uint_as_float(x)));
+}
+__device__ __forceinline__ float min_score(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+// Sum without a product ahead of it fused in.
+__device__ __forceinline__ float rounded_sum(float a, float b) {
+#pragma clang fp contract(off)
+  return a + b;
+}
+// x / 15, correctly rounded (the residual of a quotient that is off by an ulp at most, times the rounded reciprocal:
+// Markstein's correction), where the result is not subnormal; fp16 makes zero of those.
+__device__ __forceinline__ float div15(float x) {
+  const float q = x * (1.f / 15.f);
+  return fmaf(fmaf(-15.f, q, x), 1.f / 15.f, q);
+}
+// 1 / s of an fp16 value, correctly rounded the same way (held against the division for every fp16 number).
+__device__ __forceinline__ float reciprocal(float s) {
+  const float r = __builtin_amdgcn_rcpf(s);
+  return fmaf(fmaf(-s, r, 1.f), r, r);
+}
+
+// K and V: one lane per 8 dims of a row, D / 8 lanes (4 to 16) per row, the rows of 4 consecutive tokens side by side (16 to 64
+// lanes, never across a wave). A rotated row's lanes all load before any stores, so k may be rotated in place. The codes are
+// taken from the rotated values rounded to the rows' type, what a 16-bit cache would hold. Where the 4 tokens fill a quad of a V
+// tile (a prompt's do), their lanes exchange bytes and store whole words. q rows go to workgroups of their own.
 template <int DT, int D, bool INTERLEAVED>
-__global__ __launch_bounds__(256) void append_int4_kernel(Int4Append a) {
+__global__ __launch_bounds__(256) void append_int4_kernel(Int4Append a, RotaryAppend q) {
+  if (blockIdx.x >= a.blocks) {
+    rotate_rows<DT, INTERLEAVED>(q, (blockIdx.x - a.blocks) * 256u + threadIdx.x, (gridDim.x - a.blocks) * 256u);
+    return;
+  }
   constexpr int LPR = D / 8;
-  for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < a.total; i += gridDim.x * 256u) {
-    const uint32_t n = udiv(i, a.per_tok);
-    const uint32_t u = i - n * a.per_tok.d;
-    const int c = (int)(u % LPR);
-    const int head = (int)(u / LPR);
-    const int section = head < a.kv_heads ? 0 : (head < 2 * a.kv_heads ? 1 : 2);
-    const int h = head - section * a.kv_heads;
-    const Rows src = section == 0 ? a.k : (section == 1 ? a.v : a.q);
+  for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < a.total; i += a.blocks * 256u) {
+    const uint32_t n4 = udiv(i, a.per_quad);
+    const uint32_t u = i - n4 * a.per_quad.d;
+    const int c = (int)(u % LPR), k = (int)(u / LPR % 4);
+    const int head = (int)(u / (4 * LPR));
+    const bool there = 4 * n4 + k < a.n;  // the last quad may be short: its missing rows are computed and not stored
+    const uint32_t n = min(4 * n4 + k, a.n - 1);
+    const bool is_v = head >= a.kv_heads;
+    const int h = is_v ? head - a.kv_heads : head;
+    const Rows src = is_v ? a.v : a.k;
     const char* row = src.p + (int64_t)n * src.sn + (int64_t)h * src.sh;
+    const int64_t slot = a.slots[n];
     float f[8];
     load8<DT>(row, c, f);
     bool known = true;
-    if (section != 1 && a.r.table) {
+    if (a.r.table) {
       const int64_t pos = a.r.positions[n];
       known = pos >= 0 && pos < a.r.num_positions;
-      const int half = a.r.rot / 2;
-      if (known && 8 * c < a.r.rot) {
-        const float* t = a.r.table + pos * a.r.rot;
-        if constexpr (INTERLEAVED) {
-          float cs[4], sn[4];
-          load_floats<4>(t + 4 * c, cs);
-          load_floats<4>(t + half + 4 * c, sn);
+      if (!is_v) {
+        const int half = a.r.rot / 2;
+        if (known && 8 * c < a.r.rot) {
+          const float* t = a.r.table + pos * a.r.rot;
+          if constexpr (INTERLEAVED) {
+            float cs[4], sn[4];
+            load_floats<4>(t + 4 * c, cs);
+            load_floats<4>(t + half + 4 * c, sn);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) rotate_pair(f[2 * e], f[2 * e + 1], cs[e], sn[e]);
-        } else {
-          const bool low = 8 * c < half;
-          const int j = low ? c : c - half / 8;
-          float cs[8], sn[8], g[8];
-          load8<DT>(row, low ? c + half / 8 : j, g);
-          load_floats<8>(t + 8 * j, cs);
-          load_floats<8>(t + half + 8 * j, sn);
+            for (int e = 0; e < 4; ++e) rotate_pair(f[2 * e], f[2 * e + 1], cs[e], sn[e]);
+          } else {
+            const bool low = 8 * c < half;
+            const int j = low ? c : c - half / 8;
+            float cs[8], sn[8], g[8];
+            load8<DT>(row, low ? c + half / 8 : j, g);
+            load_floats<8>(t + 8 * j, cs);
+            load_floats<8>(t + half + 8 * j, sn);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float x = low ? f[e] : g[e], y = low ? g[e] : f[e];
-            rotate_pair(x, y, cs[e], sn[e]);
-            f[e] = low ? x : y;
+            for (int e = 0; e < 8; ++e) {
+              float x = low ? f[e] : g[e], y = low ? g[e] : f[e];
+              rotate_pair(x, y, cs[e], sn[e]);
+              f[e] = low ? x : y;
+            }
           }
+          round8<DT>(f);
         }
-        round8<DT>(f);
-      }
-      if (!known) {
+        if (!known) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = 0.f;
+          for (int e = 0; e < 8; ++e) f[e] = 0.f;
+        }
+        if (a.ko.p && there) store8<DT>(const_cast<char*>(a.ko.p) + (int64_t)n * a.ko.sn + (int64_t)h * a.ko.sh, c, f);
       }
-      const Rows dst = section == 0 ? a.ko : a.qo;
-      if (dst.p) store8<DT>(const_cast<char*>(dst.p) + (int64_t)n * dst.sn + (int64_t)h * dst.sh, c, f);
-    } else if (section == 1 && a.r.table) {
-      const int64_t pos = a.r.positions[n];
-      known = pos >= 0 && pos < a.r.num_positions;
     }
-    if (section == 2) continue;
-    // The group's range, over its 4 lanes.
-    float lo = __builtin_huge_valf(), hi = kNegInf;
+    // The group's range, over its 4 lanes. NaN carries through these, so one test finds what has to be taken in first.
+    float lo = f[0], hi = f[0];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      f[e] = f[e] != f[e] ? 0.f : fminf(fmaxf(f[e], -kLimit), kLimit);
-      lo = fminf(lo, f[e]);
-      hi = fmaxf(hi, f[e]);
+    for (int e = 1; e < 8; ++e) {
+      lo = min_score(lo, f[e]);
+      hi = max_score(hi, f[e]);
     }
-    lo = fminf(lo, xor_lane<1>(lo));
-    hi = fmaxf(hi, xor_lane<1>(hi));
-    lo = fminf(lo, xor_lane<2>(lo));
-    hi = fmaxf(hi, xor_lane<2>(hi));
-    const int64_t slot = a.slots[n];
-    if (!known || slot < 0 || slot >= a.num_slots) continue;
+    if (__builtin_amdgcn_ballot_w64(!(lo >= -kLimit && hi <= kLimit)) != 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f[e] = f[e] != f[e] ? 0.f : fminf(fmaxf(f[e], -kLimit), kLimit);
+        lo = e == 0 ? f[0] : fminf(lo, f[e]);
+        hi = e == 0 ? f[0] : fmaxf(hi, f[e]);
+      }
+    }
+    lo = min_score(lo, xor_lane<1>(lo));
+    hi = max_score(hi, xor_lane<1>(hi));
+    lo = min_score(lo, xor_lane<2>(lo));
+    hi = max_score(hi, xor_lane<2>(hi));
     const uint32_t low_h = to_half_bits(lo);
     const float low = half_bits(low_h);
-    const uint32_t scale_h = to_half_bits(fmaxf((hi - low) / 15.f, 0.f));
+    const uint32_t scale_h = to_half_bits(fmaxf(div15(hi - low), 0.f));
     const float scale = half_bits(scale_h);
-    const float inv = scale > 0.f ? 1.f / scale : 0.f;
+    const float inv = scale > 0.f ? reciprocal(scale) : 0.f;
+    // round((x - low) / scale) in the low bits of 1.5 * 2^23 + it, clamped there as integers; words of 8 are sums, the constant
+    // part taken off at the end.
+    constexpr uint32_t kBase = 0x4b400000u, kBases = kBase * 0x11111111u;
     uint32_t code[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) code[e] = (uint32_t)fminf(fmaxf(rintf((f[e] - low) * inv), 0.f), 15.f);
+    for (int e = 0; e < 8; ++e) {
+      const int bits = __float_as_int(rounded_sum((f[e] - low) * inv, 12582912.f));
+      code[e] = (uint32_t)min(max(bits, (int)kBase), (int)kBase + 15);
+    }
+    uint32_t word;
+    if (is_v)  // byte y: dims 2y, 2y + 1
+      word = code[0] + (code[1] << 4) + (code[2] << 8) + (code[3] << 12) + (code[4] << 16) + (code[5] << 20) +
+             (code[6] << 24) + (code[7] << 28) - kBases;
+    else
+      word = code[0] + (code[2] << 4) + (code[4] << 8) + (code[6] << 12) + (code[1] << 16) + (code[3] << 20) +
+             (code[5] << 24) + (code[7] << 28) - kBases;
+    const uint32_t meta = scale_h | low_h << 16;
+    const bool stored = there && known && slot >= 0 && slot < a.num_slots;
+    // Token k's byte y of a V word to lane y's byte k, over the lanes of the 4 tokens; and the (scale, low) of tokens k, k + 2.
+    const uint32_t far = xor_bits<2 * LPR>(word);
+    const uint32_t half = __builtin_amdgcn_perm(far, word, k < 2 ? 0x05040100u : 0x03020706u);
+    const uint32_t near = xor_bits<LPR>(half);
+    const uint32_t quad_word = __builtin_amdgcn_perm(near, half, (k & 1) == 0 ? 0x06020400u : 0x03070105u);
+    const uint32_t meta2 = xor_bits<2 * LPR>(meta);
+    // Whether the 4 tokens go to the 4 places of one quad in their order.
+    const uint32_t key = stored && ((uint32_t)slot & 3u) == (uint32_t)k ? (uint32_t)(slot >> 2) : ~(uint32_t)k;
+    const uint32_t key2 = xor_bits<2 * LPR>(key);
+    const bool whole = key == key2 && key == xor_bits<LPR>(key) && key == xor_bits<LPR>(key2);
+    if (!stored) continue;
     // slot = (block * tiles + tile of the block) * 16 + token; a (block, head) has tiles.d tiles.
-    const int64_t tile = slot >> 4;
+    const uint32_t tile = (uint32_t)(slot >> 4);
     const int t = (int)(slot & 15);
-    const int64_t blk = tile / a.tiles.d;
-    const int64_t at = ((blk * a.kv_heads + h) * a.tiles.d + (tile - blk * a.tiles.d)) * (10 * D);
-    if (section == 0) {
+    const uint32_t blk = udiv(tile, a.tiles);
+    const int64_t at = (((int64_t)blk * a.kv_heads + h) * a.tiles.d + (tile - blk * a.tiles.d)) * (10 * D);
+    if (!is_v) {
       char* o = a.k_pool + at;
-      const uint32_t w = code[0] | code[2] << 4 | code[4] << 8 | code[6] << 12 | code[1] << 16 | code[3] << 20 |
-                         code[5] << 24 | code[7] << 28;
-      *reinterpret_cast<uint32_t*>(o + t * (D / 2) + 4 * c) = w;
-      if ((c & 3) == 0) *reinterpret_cast<uint32_t*>(o + 8 * D + (t * (D / kGroup) + c / 4) * 4) = scale_h | low_h << 16;
+      *reinterpret_cast<uint32_t*>(o + t * (D / 2) + 4 * c) = word;
+      if ((c & 3) == 0) *reinterpret_cast<uint32_t*>(o + 8 * D + (t * (D / kGroup) + c / 4) * 4) = meta;
     } else {
       char* o = a.v_pool + at;
-      const int quad = t >> 2, k = t & 3;
+      const int quad = t >> 2;
+      char* data = o + quad * 2 * D + 16 * c;
+      char* m = o + 8 * D + (quad * (D / kGroup) + c / 4) * 16;
+      if (whole) {
+        *reinterpret_cast<uint32_t*>(data + 4 * k) = quad_word;
+        if ((c & 3) == 0 && k < 2) {  // tokens 0, 2 and 1, 3
+          *reinterpret_cast<uint32_t*>(m + 4 * k) = __builtin_amdgcn_perm(meta2, meta, 0x05040100u);
+          *reinterpret_cast<uint32_t*>(m + 8 + 4 * k) = __builtin_amdgcn_perm(meta2, meta, 0x07060302u);
+        }
+      } else {
+        const int tk = t & 3;
 #pragma unroll
-      for (int y = 0; y < 4; ++y)
-        o[quad * 2 * D + (4 * c + y) * 4 + k] = (char)(code[2 * y] | code[2 * y + 1] << 4);
-      if ((c & 3) == 0) {
-        char* m = o + 8 * D + (quad * (D / kGroup) + c / 4) * 16 + 2 * ((k & 1) * 2 + (k >> 1));
-        *reinterpret_cast<uint16_t*>(m) = (uint16_t)scale_h;
-        *reinterpret_cast<uint16_t*>(m + 8) = (uint16_t)low_h;
+        for (int y = 0; y < 4; ++y) data[4 * y + tk] = (char)(word >> (8 * y));
+        if ((c & 3) == 0) {
+          m += 2 * ((tk & 1) * 2 + (tk >> 1));
+          *reinterpret_cast<uint16_t*>(m) = (uint16_t)scale_h;
+          *reinterpret_cast<uint16_t*>(m + 8) = (uint16_t)low_h;
+        }
       }
     }
   }
@@ -187,7 +253,7 @@ __global__ __launch_bounds__(256) void append_int4_kernel(Int4Append a) {
 template <int DT, int D>
 __global__ __launch_bounds__(256) void gather_int4_kernel(const char* k_pool, const char* v_pool, const int32_t* tables,
                                                           int64_t tstride, const int32_t* lens, char* k_out, char* v_out,
-                                                          uint32_t total, DivU32 quads, DivU32 heads, int32_t tiles,
+                                                          uint32_t total, DivU32 quads, DivU32 heads, DivU32 tiles,
                                                           int32_t nb, int32_t max_len) {
   constexpr int LPR = D / 8;
   constexpr int kRow = D * (DT == SKV_F32 ? 4 : 2);
@@ -207,10 +273,10 @@ __global__ __launch_bounds__(256) void gather_int4_kernel(const char* k_pool, co
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[k][e] = 0.f;
     if (t0 < len) {
-      const int tile = t0 >> 4, in = tile % tiles, blk_i = tile / tiles;
+      const uint32_t tile = (uint32_t)t0 >> 4, blk_i = udiv(tile, tiles), in = tile - blk_i * tiles.d;
       const uint32_t blk = (uint32_t)tables[(int64_t)b * tstride + blk_i];
       if (blk < (uint32_t)nb) {
-        const char* p = (is_v ? v_pool : k_pool) + (((int64_t)blk * heads.d + h) * tiles + in) * (10 * D);
+        const char* p = (is_v ? v_pool : k_pool) + (((int64_t)blk * heads.d + h) * tiles.d + in) * (10 * D);
         const int t = t0 & 15, quad = t >> 2;
         if (!is_v) {
 #pragma unroll
@@ -934,22 +1000,25 @@ void launch_attn4_d(int d, const Int4Attn& p, hipStream_t stream) {
     launch_attn4<DT, 128>(p, stream);
 }
 
+uint32_t blocks_of(uint32_t total) { return (uint32_t)(cdiv(total, 256) < 32767 ? cdiv(total, 256) : 32767); }
+
 template <int DT, int D>
-void launch_append4(const Int4Append& a, hipStream_t stream) {
-  const uint32_t blocks = (uint32_t)(cdiv(a.total, 256) < 65535 ? cdiv(a.total, 256) : 65535);
+void launch_append4(Int4Append a, const RotaryAppend& q, hipStream_t stream) {
+  a.blocks = blocks_of(a.total);
+  const dim3 grid(a.blocks + blocks_of(q.total));
   if (a.r.interleaved)
-    hipLaunchKernelGGL((append_int4_kernel<DT, D, true>), dim3(blocks), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((append_int4_kernel<DT, D, true>), grid, dim3(256), 0, stream, a, q);
   else
-    hipLaunchKernelGGL((append_int4_kernel<DT, D, false>), dim3(blocks), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((append_int4_kernel<DT, D, false>), grid, dim3(256), 0, stream, a, q);
 }
 template <int DT>
-void launch_append4_d(int d, const Int4Append& a, hipStream_t stream) {
+void launch_append4_d(int d, const Int4Append& a, const RotaryAppend& q, hipStream_t stream) {
   if (d == 32)
-    launch_append4<DT, 32>(a, stream);
+    launch_append4<DT, 32>(a, q, stream);
   else if (d == 64)
-    launch_append4<DT, 64>(a, stream);
+    launch_append4<DT, 64>(a, q, stream);
   else
-    launch_append4<DT, 128>(a, stream);
+    launch_append4<DT, 128>(a, q, stream);
 }
 
 struct Int4Gather {
@@ -959,8 +1028,8 @@ struct Int4Gather {
   const int32_t* lens;
   char *k_out, *v_out;
   uint32_t total;
-  DivU32 quads, heads;
-  int32_t tiles, nb, max_len;
+  DivU32 quads, heads, tiles;
+  int32_t nb, max_len;
 };
 template <int DT, int D>
 void launch_gather4(const Int4Gather& a, hipStream_t stream) {
@@ -984,6 +1053,7 @@ int check_pool(const char* who, const void* k_pool, const void* v_pool, int32_t 
   if (kv_heads <= 0 || kv_heads > 65535 || nb < 0 || bs <= 0 || bs % kTile)
     return fail(SKV_EINVAL, "%s: bad pool kv_heads=%d num_blocks=%lld block_size=%d (a multiple of %d)", who, kv_heads,
                 (long long)nb, bs, kTile);
+  if (nb * (bs / kTile) > (int64_t)1 << 29) return fail(SKV_EINVAL, "%s: pool of %lld x %d tokens is too large", who, (long long)nb, bs);
   if (!k_pool || !v_pool) return fail(SKV_EINVAL, "%s: null pool", who);
   if (!aligned16(k_pool) || !aligned16(v_pool)) return fail(SKV_EALIGN, "%s: pools must be 16-byte aligned", who);
   return SKV_OK;
@@ -1020,35 +1090,46 @@ int skv_append_int4(const void* q, int64_t q_stride_n, int64_t q_stride_h, const
   if (k_out) odd |= ko_stride_n | ko_stride_h;
   if (odd % (16 / eb)) return fail(SKV_EALIGN, "%s: strides must be multiples of %d elements", who, 16 / eb);
   Int4Append a{};
-  const int64_t lanes = ((q ? num_heads : 0) + 2 * (int64_t)num_kv_heads) * (head_dim / 8);
-  if (lanes >= (int64_t)1 << 30) return fail(SKV_EINVAL, "%s: too many heads", who);
-  a.per_tok = make_div((uint32_t)lanes);
+  RotaryAppend qa{};  // q rows alone: no K or V heads
+  const int epl = 16 / eb;
+  const int64_t lanes = 2 * (int64_t)num_kv_heads * (head_dim / 8), pairs = head_dim / (2 * epl);
+  const int64_t q_pairs = q ? num_heads * pairs : 1;
+  if (lanes >= (int64_t)1 << 28 || q_pairs >= (int64_t)1 << 28) return fail(SKV_EINVAL, "%s: too many heads", who);
+  a.per_quad = make_div((uint32_t)(4 * lanes));
   a.tiles = make_div((uint32_t)(block_size / kTile));
-  a.q_heads = q ? num_heads : 0;
   a.kv_heads = num_kv_heads;
   a.k_pool = (char*)k_pool;
   a.v_pool = (char*)v_pool;
   a.num_slots = (int64_t)num_blocks * block_size;
   a.r = {cos_sin, positions, num_positions, rot_dim, interleaved ? 1 : 0};
+  qa.per_tok = make_div((uint32_t)q_pairs);
+  qa.pairs = make_div((uint32_t)pairs);
+  qa.q_heads = q ? num_heads : 0;
+  qa.r = a.r;
   // Indices of a launch stay below 2^31: longer batches go in slices of tokens.
-  const int64_t slice = (((int64_t)1 << 31) - 1) / lanes;
+  const int64_t most = 4 * lanes > q_pairs ? 4 * lanes : q_pairs;
+  const int64_t slice = (((int64_t)1 << 31) - 1) / most * 4;
   for (int64_t n0 = 0; n0 < n_tokens; n0 += slice) {
     const int64_t n = n_tokens - n0 < slice ? n_tokens - n0 : slice;
     auto rows = [&](const void* p, int64_t sn, int64_t sh) {
       return Rows{p ? (const char*)p + n0 * sn * eb : nullptr, sn * eb, sh * eb};
     };
-    a.q = rows(q, q_stride_n, q_stride_h);
     a.k = rows(k_new, k_stride_n, k_stride_h);
     a.v = rows(v_new, v_stride_n, v_stride_h);
-    a.qo = rows(q_out, qo_stride_n, qo_stride_h);
     a.ko = rows(k_out, ko_stride_n, ko_stride_h);
-    a.slots = slot_mapping + n0;
-    a.r.positions = positions ? positions + n0 : nullptr;
-    a.total = (uint32_t)(n * lanes);
+    a.slots = qa.slots = slot_mapping + n0;
+    a.r.positions = qa.r.positions = positions ? positions + n0 : nullptr;
+    a.n = (uint32_t)n;
+    a.total = (uint32_t)(cdiv(n, 4) * 4 * lanes);
+    if (q) {
+      qa.q = rows(q, q_stride_n, q_stride_h);
+      qa.qo = rows(q_out, qo_stride_n, qo_stride_h);
+      qa.total = (uint32_t)(n * q_pairs);
+    }
     switch (dtype) {
-      case SKV_F32: launch_append4_d<SKV_F32>(head_dim, a, (hipStream_t)stream); break;
-      case SKV_F16: launch_append4_d<SKV_F16>(head_dim, a, (hipStream_t)stream); break;
-      default: launch_append4_d<SKV_BF16>(head_dim, a, (hipStream_t)stream); break;
+      case SKV_F32: launch_append4_d<SKV_F32>(head_dim, a, qa, (hipStream_t)stream); break;
+      case SKV_F16: launch_append4_d<SKV_F16>(head_dim, a, qa, (hipStream_t)stream); break;
+      default: launch_append4_d<SKV_BF16>(head_dim, a, qa, (hipStream_t)stream); break;
     }
     rc = check_launch(who);
     if (rc != SKV_OK) return rc;
@@ -1078,7 +1159,7 @@ int skv_gather_int4(const void* k_pool, const void* v_pool, const int32_t* block
     const int64_t n = batch - b0 < slice ? batch - b0 : slice;
     const Int4Gather a{(const char*)k_pool, (const char*)v_pool, block_tables + b0 * table_stride, table_stride, lens + b0,
                        (char*)k_out + b0 * out_bytes, (char*)v_out + b0 * out_bytes, (uint32_t)(n * per_row),
-                       make_div((uint32_t)quads), make_div((uint32_t)num_kv_heads), block_size / kTile, num_blocks, max_len};
+                       make_div((uint32_t)quads), make_div((uint32_t)num_kv_heads), make_div((uint32_t)(block_size / kTile)), num_blocks, max_len};
     switch (dtype) {
       case SKV_F32: launch_gather4_d<SKV_F32>(head_dim, a, (hipStream_t)stream); break;
       case SKV_F16: launch_gather4_d<SKV_F16>(head_dim, a, (hipStream_t)stream); break;

@@ -88,6 +88,29 @@ def test_append_extremes(cuda):
         assert torch.isfinite(gk).all() and torch.isfinite(gv).all()
 
 
+def test_append_every_scale(cuda):
+    """Groups of every fp16 scale up to the greatest the cache takes, its codes' borders among the elements: what the kernel's
+    quotient and reciprocal give is what division gives."""
+    scales = np.arange(1, 0x7c00, dtype=np.uint16).view(np.float16).astype(np.float32)
+    scales = scales[scales <= 2184]
+    n = -(-len(scales) // 8)
+    scales = np.concatenate([scales, np.ones(n * 8 - len(scales), np.float32)])
+    rng = np.random.default_rng(0)
+    x = (rng.random((n * 8, 32), np.float32) * 15).astype(np.float32)
+    x[:, 2:18] = np.arange(16) + np.where(np.arange(16) < 15, 0.5, 0)  # the borders between codes
+    x[:, 0], x[:, 1] = 0, 15
+    x = (x * scales[:, None] + rng.integers(-1, 2, (n * 8, 1)) * scales[:, None]).astype(np.float32).reshape(n, 8, 32)
+    k = torch.from_numpy(x).cuda()
+    blocks = -(-n // 16)
+    kp, vp = pools(blocks, 16, 8, 32)
+    native.append_int4(k, k, kp, vp, torch.arange(n, device="cuda"))
+    code, scale, low = ic.quantise(x)
+    want = torch.from_numpy(ic.values(code, scale, low)).float()
+    table = torch.arange(blocks, dtype=torch.int32, device="cuda").view(1, -1)
+    for got in native.gather_int4(kp, vp, table, torch.tensor([n], dtype=torch.int32, device="cuda"), n, torch.float32):
+        assert torch.equal(got[0].transpose(0, 1).cpu(), want)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("inter,rot", [(False, 128), (True, 128), (False, 32), (True, 16)])
 def test_append_rotated(cuda, dtype, inter, rot):
