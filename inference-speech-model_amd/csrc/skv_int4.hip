@@ -1107,8 +1107,8 @@ int skv_append_int4(const void* q, int64_t q_stride_n, int64_t q_stride_h, const
   qa.q_heads = q ? num_heads : 0;
   qa.r = a.r;
   // Indices of a launch stay below 2^31: longer batches go in slices of tokens.
-  const int64_t most = 4 * lanes > q_pairs ? 4 * lanes : q_pairs;
-  const int64_t slice = (((int64_t)1 << 31) - 1) / most * 4;
+  const int64_t most = lanes > q_pairs ? lanes : q_pairs;
+  const int64_t slice = (((int64_t)1 << 31) - 1) / (4 * most) * 4;
   for (int64_t n0 = 0; n0 < n_tokens; n0 += slice) {
     const int64_t n = n_tokens - n0 < slice ? n_tokens - n0 : slice;
     auto rows = [&](const void* p, int64_t sn, int64_t sh) {
@@ -1210,6 +1210,8 @@ int skv_paged_attention_int4(const void* q, int64_t q_stride_b, int64_t q_stride
   if (max_ctx > cap) max_ctx = (int32_t)cap;
   if (chunk_tokens <= 0)
     chunk_tokens = skv_int4_chunk_tokens(batch, q_len, num_heads, num_kv_heads, head_dim, max_ctx, dtype);
+  if (max_ctx > 1 << 30 || chunk_tokens > 1 << 30)
+    return fail(SKV_EINVAL, "%s: max_ctx %d or chunk_tokens %d past 2^30", who, max_ctx, chunk_tokens);
   if (chunk_tokens % kChunkUnit)
     return fail(SKV_EINVAL, "%s: chunk_tokens %d must be a multiple of %d", who, chunk_tokens, kChunkUnit);
   Int4Attn p{};

@@ -78,7 +78,8 @@ ATTN = dict(q=P, qb=512, qq=512, qh=64, kp=P, vp=P, tables=P, stride=40, rows=No
     (dict(lens=None), EINVAL, b"null"), (dict(tables=None), EINVAL, b"null"), (dict(o=P + 2), EALIGN, b"align"),
     (dict(qh=60), EALIGN, b"stride"), (dict(chunk=96), EINVAL, b"chunk"), (dict(ws=None), EWORKSPACE, b"workspace"),
     (dict(ws_bytes=100), EWORKSPACE, b"workspace"), (dict(ws=P + 8), EWORKSPACE, b"workspace"),
-    (dict(b=1 << 22), EINVAL, b"too large")])
+    (dict(b=1 << 22), EINVAL, b"too large"), (dict(nb=1 << 30), EINVAL, b"too large"),
+    (dict(stride=1 << 27, max_ctx=(1 << 30) + 1), EINVAL, b"past"), (dict(chunk=(1 << 30) + 64), EINVAL, b"past")])
 def test_paged_attention_int4_entry(lib, change, code, word):
     rc = lib.skv_paged_attention_int4(*{**ATTN, **change}.values(), None)
     assert rc == code and word in lib.skv_last_error(), lib.skv_last_error()
