@@ -559,18 +559,24 @@ struct Words {
   uint32_t w[N];
 };
 template <int N>
-__device__ __forceinline__ Words<N> load_words(const char* p) {
+__device__ __forceinline__ Words<N> load_words(__amdgpu_buffer_rsrc_t tile, uint32_t off) {
   Words<N> r;
   if constexpr (N == 4) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint4 v = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(tile, off, 0, 0));
     r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
   } else if constexpr (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    const uint2 v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(tile, off, 0, 0));
     r.w[0] = v.x, r.w[1] = v.y;
   } else {
-    r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+    r.w[0] = __builtin_amdgcn_raw_buffer_load_b32(tile, off, 0, 0);
   }
   return r;
+}
+
+// One tile of a pool: loads at 32-bit lane offsets from a scalar base (with plain pointers the compiler kept the sums of pool and
+// lane offset, two vector registers each, and added the tile's offset to them every step).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_at(const char* pool, uint64_t at, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(pool + at), (short)0, bytes, kBufWord3);
 }
 
 // What a wave holds of one step: two 16-key tiles.
@@ -603,7 +609,7 @@ __device__ __forceinline__ float max_groups(float x) {
 }
 
 template <int DT, int D>
-__global__ __launch_bounds__(64 * kAttnWaves, D == 128 ? 3 : 4) void attention_int4_mfma_kernel(Int4Attn p, Int4Divs dv) {
+__global__ __launch_bounds__(64 * kAttnWaves, D == 128 ? 4 : 5) void attention_int4_mfma_kernel(Int4Attn p, Int4Divs dv) {
   constexpr int WAVES = kAttnWaves;
   constexpr int ND = D / 32;
   constexpr int NB = D / 16;     // 16-row blocks of the result
@@ -664,18 +670,18 @@ __global__ __launch_bounds__(64 * kAttnWaves, D == 128 ? 3 : 4) void attention_i
   auto load_k = [&](const Tiles& t) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const char* k = p.k_pool + t.at[i];
-      cur.k[i] = load_words<ND>(k + k_off);
-      cur.ks[i] = *reinterpret_cast<const uint32_t*>(k + ks_off);
-      cur.kr[i] = *reinterpret_cast<const uint32_t*>(k + kr_off);
+      const __amdgpu_buffer_rsrc_t k = tile_at(p.k_pool, t.at[i], 10 * D);
+      cur.k[i] = load_words<ND>(k, k_off);
+      cur.ks[i] = load_words<1>(k, ks_off).w[0];
+      cur.kr[i] = load_words<1>(k, kr_off).w[0];
     }
   };
   auto load_v = [&](const Tiles& t) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const char* v = p.v_pool + t.at[i];
-      cur.v[i] = load_words<ND>(v + v_off);
-      cur.vm[i] = *reinterpret_cast<const uint4*>(v + vm_off);
+      const __amdgpu_buffer_rsrc_t v = tile_at(p.v_pool, t.at[i], 10 * D);
+      cur.v[i] = load_words<ND>(v, v_off);
+      cur.vm[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(v, vm_off, 0, 0));
     }
   };
   // The registers of a step's K take the next step's as soon as they are read, and V's theirs: each load has the other
@@ -966,13 +972,21 @@ int64_t attn4_items(int32_t batch, int32_t q_len, int32_t heads, int32_t kv_head
   return (int64_t)batch * cdiv((int64_t)(heads / kv_heads) * q_len, 16) * kv_heads;
 }
 
-// Key chunk of a call of `items` workgroups before its keys are split.
-int32_t pick_chunk4(int64_t items, int32_t d, int32_t max_ctx) {
-  const int64_t units = cdiv(max_ctx > 0 ? max_ctx : 1, kChunkUnit);
-  int64_t chunks = max_ctx <= 512 || items >= (d == 128 ? 512 : 1024) ? 1 : 1024 / (items > 0 ? items : 1);
-  const int64_t most = cdiv(units, 2);
-  chunks = chunks > most ? most : (chunks < 1 ? 1 : chunks);
-  return (int32_t)(cdiv(units, chunks) * kChunkUnit);
+// Key chunk of a call of `items` workgroups before its keys are split: none for short rows (the second launch that joins the
+// parts costs 2.5 us) and many items; else one workgroup per compute unit, of 128 to 1024 keys. bf16, one request of
+// 8 / 20 KV heads x 128 / 64, us by chunk (the rule's in brackets):
+//   8 x 2000 keys     [128] 8.8   256 9.4   512 11.1  unsplit 19.0
+//   8 x 8000          128 11.7  [256] 9.7   512 11.5  1024 14.7
+//   8 x 32000         256 20.1   512 18.1 [1024] 17.4  2048 24.4
+//   20 x 600 (64)     128 7.8    256 8.3   512 9.6    [unsplit] 7.4
+//   128 x 1000        256 12.5   512 12.0  [unsplit] 12.2;  320 x 1000 (64) 256 14.2  512 14.2  [unsplit] 12.7
+//   256 x 1000..16384 512 95.9 [1024] 87.8  2048 85.8  4096 96.5;  512 x 200..2000 512 31.1  1024 31.4  [unsplit] 28.0
+int32_t pick_chunk4(int64_t items, int32_t max_ctx) {
+  const int64_t ctx = max_ctx > 0 ? max_ctx : 1;
+  if (ctx <= 768 || (ctx <= 1024 && items >= 128) || (ctx <= 2048 && items >= 512))
+    return (int32_t)(cdiv(ctx, kChunkUnit) * kChunkUnit);
+  const int64_t even = cdiv(items * ctx / 256, kChunkUnit) * kChunkUnit;
+  return (int32_t)(even < 128 ? 128 : (even > 1024 ? 1024 : even));
 }
 
 template <int DT, int D>
@@ -1174,7 +1188,7 @@ int skv_gather_int4(const void* k_pool, const void* v_pool, const int32_t* block
 int32_t skv_int4_chunk_tokens(int32_t batch, int32_t q_len, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                               int32_t max_ctx, int32_t dtype) {
   if (batch <= 0 || q_len <= 0 || num_heads <= 0 || num_kv_heads <= 0) return kChunkUnit;
-  return pick_chunk4(attn4_items(batch, q_len, num_heads, num_kv_heads, dtype), head_dim, max_ctx);
+  return pick_chunk4(attn4_items(batch, q_len, num_heads, num_kv_heads, dtype), max_ctx);
 }
 
 int64_t skv_int4_workspace_bytes(int32_t batch, int32_t q_len, int32_t num_heads, int32_t head_dim, int32_t max_ctx,
