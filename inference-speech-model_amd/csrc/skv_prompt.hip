@@ -86,36 +86,55 @@ __device__ __forceinline__ uint2 lds_tr16(const char* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4) const_cast<char*>(p)));
 }
 
-// The (sequence, query tile) of a work index: sequences have ceil(length / M) tiles each. False past the last one.
+__device__ __forceinline__ float wave_max(float x) {
+  x = fmaxf(x, xor_lane<1>(x));
+  x = fmaxf(x, xor_lane<2>(x));
+  x = fmaxf(x, xor_lane<4>(x));
+  x = fmaxf(x, xor_lane<8>(x));
+  x = fmaxf(x, xor_lane<16>(x));
+  return fmaxf(x, xor_lane<32>(x));
+}
+
+// The (sequence, query tile) of a work index: sequences have ceil(length / M) tiles each, and tiles with more keys come first
+// (within each 64 sequences), so that the workgroups that take longest do not start last. False past the last tile.
 template <int M>
 __device__ __forceinline__ bool find_tile(const PromptAttn& p, int index, int& begin, int& len, int& tile) {
   const int lane = threadIdx.x & 63;
-  int run = 0;
   for (int s0 = 0; s0 < p.seqs; s0 += 64) {
     int b = 0, e = 0;
     if (s0 + lane < p.seqs) seq_range(p, s0 + lane, b, e);
     const int n = (e - b + M - 1) / M;
-    int sum = n;  // inclusive prefix sum over the lanes
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int up = __shfl_up(sum, o);
-      if (lane >= o) sum += up;
+    // Tiles with a number of t or more, over the 64 sequences (fewer than 2^24 in a launch, which floats count).
+    auto from = [&](int t) __attribute__((always_inline)) {
+      return __builtin_amdgcn_readfirstlane((int)group_sum<64>((float)max(n - t, 0)));
+    };
+    const int all = from(0);
+    if (index >= all) {
+      index -= all;
+      continue;
     }
-    const uint64_t behind = __builtin_amdgcn_ballot_w64(run + sum > index);
-    if (behind) {
-      const int l = __builtin_ctzll(behind);
-      begin = __builtin_amdgcn_readlane(b, l);
-      len = __builtin_amdgcn_readlane(e, l) - begin;
-      tile = index - (run + __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l));
-      return true;
+    int lo = 0, hi = __builtin_amdgcn_readfirstlane((int)wave_max((float)n)), ahead = 0;
+    while (hi - lo > 1) {  // from(lo) > index >= from(hi) = ahead
+      const int mid = (lo + hi) / 2, f = from(mid);
+      if (f > index)
+        lo = mid;
+      else
+        hi = mid, ahead = f;
     }
-    run += __builtin_amdgcn_readlane(sum, 63);
+    // The (index - ahead)-th sequence of those that have a tile number lo.
+    const uint64_t have = __builtin_amdgcn_ballot_w64(n > lo);
+    const int before = __builtin_popcountll(have & ((1ull << lane) - 1));
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(n > lo && before == index - ahead));
+    begin = __builtin_amdgcn_readlane(b, l);
+    len = __builtin_amdgcn_readlane(e, l) - begin;
+    tile = lo;
+    return true;
   }
   return false;
 }
 
 template <int DT, int D, int QW, int KW>
-__global__ __launch_bounds__(64 * QW * KW, 2) void prompt_kernel(PromptAttn p, int tiles) {
+__global__ __launch_bounds__(64 * QW * KW, 2) void prompt_kernel(PromptAttn p) {
   constexpr int M = 32 * QW;
   constexpr int KB = 2 / KW;                // 32-key blocks of a tile that a wave takes
   constexpr int VPR = D / 8;                // 16-byte vectors per row
@@ -135,13 +154,12 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void prompt_kernel(PromptAttn p, i
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int qw = wave % QW, kw = wave / QW;
   const int n = lane & 31, f = lane >> 5;
-  // Heads vary fastest, the heads of a die (workgroup index modulo 8) being neighbours that share K/V; tiles go from the
-  // last, which has the most keys, to the first.
+  // Heads vary fastest, the heads of a die (workgroup index modulo 8) being neighbours that share K/V.
   const int H = p.heads;
   int h = (int)(blockIdx.x % (uint32_t)H);
   if ((H & 7) == 0) h = (h & 7) * (H >> 3) + (h >> 3);
   int begin, len, tile;
-  if (!find_tile<M>(p, tiles - 1 - (int)(blockIdx.x / (uint32_t)H), begin, len, tile)) return;
+  if (!find_tile<M>(p, (int)(blockIdx.x / (uint32_t)H), begin, len, tile)) return;
   const int kvh = h / p.group;
   const int first = tile * M + qw * 32;     // the wave's first query in its sequence
   const int keys = min(len, tile * M + M);  // keys of the workgroup
@@ -365,7 +383,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void prompt_kernel(PromptAttn p, i
 constexpr int kWaves32 = 4;
 
 template <int D>
-__global__ __launch_bounds__(64 * kWaves32) void prompt_f32_kernel(PromptAttn p, int tiles) {
+__global__ __launch_bounds__(64 * kWaves32) void prompt_f32_kernel(PromptAttn p) {
   constexpr int KD = D / 4, VD = D / 16;  // floats of a lane's piece of a K row and of a V row
   __shared__ float s_ml[kWaves32][2][16];
   __shared__ float s_acc[kWaves32][16][D + 4];
@@ -374,7 +392,7 @@ __global__ __launch_bounds__(64 * kWaves32) void prompt_f32_kernel(PromptAttn p,
   const int g = lane >> 4, r = lane & 15;
   const int h = (int)(blockIdx.x % (uint32_t)p.heads);
   int begin, len, tile;
-  if (!find_tile<16>(p, tiles - 1 - (int)(blockIdx.x / (uint32_t)p.heads), begin, len, tile)) return;
+  if (!find_tile<16>(p, (int)(blockIdx.x / (uint32_t)p.heads), begin, len, tile)) return;
   const int kvh = h / p.group;
   const int first = tile * 16, keys = min(len, first + 16);
   const char* kbase = p.k + (int64_t)begin * p.ksn + (int64_t)kvh * p.ksh + g * KD * 4;
@@ -485,8 +503,7 @@ __global__ __launch_bounds__(64 * kWaves32) void prompt_f32_kernel(PromptAttn p,
 template <int DT, int D, int QW, int KW>
 void launch_tiles(const PromptAttn& p, hipStream_t stream) {
   const int tiles = p.n / (32 * QW) + p.seqs;  // at least the sum of ceil(length / M)
-  hipLaunchKernelGGL((prompt_kernel<DT, D, QW, KW>), dim3((uint32_t)tiles * (uint32_t)p.heads), dim3(64 * QW * KW), 0, stream, p,
-                     tiles);
+  hipLaunchKernelGGL((prompt_kernel<DT, D, QW, KW>), dim3((uint32_t)tiles * (uint32_t)p.heads), dim3(64 * QW * KW), 0, stream, p);
 }
 // Few workgroups (no more than the compute units) are as slow as the one with the most keys: two waves then share 32 queries'
 // keys. bf16 32 / 8 heads x 128 (us, 128 queries a workgroup / 64 with shared keys): 512 tokens (128 workgroups) 15.9 / 12.3,
@@ -501,7 +518,7 @@ void launch_prompt(const PromptAttn& p, hipStream_t stream) {
 template <int D>
 void launch_prompt_f32(const PromptAttn& p, hipStream_t stream) {
   const int tiles = p.n / 16 + p.seqs;
-  hipLaunchKernelGGL((prompt_f32_kernel<D>), dim3((uint32_t)tiles * (uint32_t)p.heads), dim3(64 * kWaves32), 0, stream, p, tiles);
+  hipLaunchKernelGGL((prompt_f32_kernel<D>), dim3((uint32_t)tiles * (uint32_t)p.heads), dim3(64 * kWaves32), 0, stream, p);
 }
 template <int DT>
 void launch_prompt_d(int d, const PromptAttn& p, hipStream_t stream) {
