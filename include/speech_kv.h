@@ -40,6 +40,10 @@
  *                         token feedback per decode slot. Replaces argmax +
  *                         copy_ at speech_serving/models.py:486-487 and
  *                         graph_decode_buffers.py:463.
+ *   skv_append_rotary, skv_append_int4, skv_gather_int4, skv_paged_attention_int4,
+ *   skv_prompt_attention  append with the position rotation on the way, the paged cache in
+ *                         4 bits, causal attention of packed prompts: beside the calls
+ *                         above, for decoders with rotary positions (described below).
  *
  * Conventions
  *   - Every pointer argument is a device pointer owned by the caller (PyTorch).
@@ -88,7 +92,7 @@ enum skv_status {
   SKV_EINVAL = -1,     /* bad size / null pointer / unsupported head_dim */
   SKV_EDTYPE = -2,     /* unknown dtype code */
   SKV_EALIGN = -3,     /* pointer or stride not 16-byte aligned */
-  SKV_EWORKSPACE = -4, /* workspace missing or smaller than skv_attention_workspace_bytes */
+  SKV_EWORKSPACE = -4, /* workspace missing or smaller than skv_attention_workspace_bytes (skv_int4_workspace_bytes) */
   SKV_EUNSUPPORTED = -5 /* skv_linear: no workspace-free hipBLASLt algorithm for the shape;
                            skv_decode_linear, skv_rows_linear: not a shape or layout they take */
 };

@@ -101,6 +101,8 @@ __device__ __forceinline__ float reciprocal(float s) {
 // lanes, never across a wave). A rotated row's lanes all load before any stores, so k may be rotated in place. The codes are
 // taken from the rotated values rounded to the rows' type, what a 16-bit cache would hold. Where the 4 tokens fill a quad of a V
 // tile (a prompt's do), their lanes exchange bytes and store whole words. q rows go to workgroups of their own.
+// What bounds it: about 210 vector operations for a lane's 8 values (range, codes, words), as much as the bytes: bf16 16000 rows
+// of 20 x 64 28-30 us (3.6-3.9 TB/s; 36 with bytes stored one by one and divisions), 8192 tokens rotated with 32 / 8 heads x 128 43 us.
 template <int DT, int D, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void append_int4_kernel(Int4Append a, RotaryAppend q) {
   if (blockIdx.x >= a.blocks) {
@@ -249,7 +251,8 @@ __global__ __launch_bounds__(256) void append_int4_kernel(Int4Append a, RotaryAp
 // ---------------------------------------------------------------------------
 // Gather: out[b, h, t, :] = the values of position t of row b for t < lens[b], zero otherwise.
 // ---------------------------------------------------------------------------
-// One thread per 8 dims of 4 tokens (a quad) of one head, of K (grid.y 0) or V (1).
+// One thread per 8 dims of 4 tokens (a quad) of one head, of K (grid.y 0) or V (1): V's words hold 4 tokens. Bound by the bytes it
+// writes: bf16 16 rows to 1500 of 20 x 64, 149 MB, 23.5 us (6.3 TB/s).
 template <int DT, int D>
 __global__ __launch_bounds__(256) void gather_int4_kernel(const char* k_pool, const char* v_pool, const int32_t* tables,
                                                           int64_t tstride, const int32_t* lens, char* k_out, char* v_out,
@@ -351,8 +354,10 @@ __device__ __forceinline__ int visible(const Int4Attn& p, int b, int qi) {
 
 // One workgroup per (row, query, head, key chunk), everything in fp32: 16-key tiles go to its waves in turn.
 // Scores: lane (g, r) takes a quarter of key r's dims. Values: lane m takes dims 2m and 2m + 1 of D / 2 lanes' worth of
-// quads. For fp32 rows, whose results are held to fp32's rounding.
-template <int DT, int D>
+// quads. For fp32 rows, whose results are held to fp32's rounding: values are low + scale * code in fp32 before their products
+// (codes first, scale after the sum, cancels: 1.4e-7 of the results' rms from float64 at 4 keys, now 0.65e-7). Bound by its vector
+// operations: 4 rows x 2000 keys, 8 heads x 64, 8.0 us.
+template <int D>
 __global__ __launch_bounds__(64 * kAttnWaves) void attention_int4_kernel(Int4Attn p) {
   constexpr int ND = D / 32;        // dwords of a lane's quarter row
   constexpr int LPM = D / 2;        // lanes that cover a row of V
@@ -374,7 +379,7 @@ __global__ __launch_bounds__(64 * kAttnWaves) void attention_int4_kernel(Int4Att
   const char* q = p.q + (int64_t)b * p.qsb + (int64_t)qi * p.qsq + (int64_t)h * p.qsh;
   if (threadIdx.x < D / 8) {
     float f[8];
-    load8<DT>(q, threadIdx.x, f);
+    load8<SKV_F32>(q, threadIdx.x, f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s_q[8 * threadIdx.x + e] = f[e];
   }
@@ -472,11 +477,7 @@ __global__ __launch_bounds__(64 * kAttnWaves) void attention_int4_kernel(Int4Att
     return;
   }
   const float out = l > 0.f || l != l ? acc / l : 0.f;
-  char* o = p.o + (int64_t)b * p.osb + (int64_t)qi * p.osq + (int64_t)h * p.osh;
-  if constexpr (DT == SKV_F32)
-    reinterpret_cast<float*>(o)[d] = out;
-  else
-    reinterpret_cast<uint16_t*>(o)[d] = (uint16_t)pack2<DT>(out, 0.f);
+  reinterpret_cast<float*>(p.o + (int64_t)b * p.osb + (int64_t)qi * p.osq + (int64_t)h * p.osh)[d] = out;
 }
 
 // 16-bit rows on the matrix cores. One workgroup per (row, KV head, 16 queries, key chunk): the queries are those of the
@@ -494,7 +495,9 @@ __global__ __launch_bounds__(64 * kAttnWaves) void attention_int4_kernel(Int4Att
 // rounded head and its rounded remainder; their sum is one more row of the product.
 // fp16, 300 keys: 2.7e-4 of the results' rms from float64, where rounding exact ones is 2.1e-4 (with K's scale in its operand
 // as well 3.6e-4, with weights rounded once 3.3e-4, with low - 16 scale rounded into the fma 25e-4).
-// What bounds it: HBM for long rows, with about 2.2 vector operations an element beside them.
+// What bounds it: HBM and the vector operations alike on long rows (about 3.3 an element at head_dim 128, half of them to unpack),
+// for few keys the chain lengths -> table -> keys -> join. bf16 unless said, 32 / 8 heads x 128: 32 rows of 1000..16384 keys 83 us
+// (4.3 TB/s), fp16 one row of 131072 keys 34 us (5.0 TB/s); 20 heads x 64: 16 x 4096 keys 27 us (3.9 TB/s), 64 rows of 1..452 keys 12.8.
 constexpr float kLazyMaxLog2 = 8.f;  // the accumulators are rescaled when a maximum grows by more than this
 constexpr float kWeightLog2 = 6.f;   // weights below 2^(8 + 6)
 
@@ -684,10 +687,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, D == 128 ? 4 : 5) void attention_i
       cur.vm[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(v, vm_off, 0, 0));
     }
   };
-  // The registers of a step's K take the next step's as soon as they are read, and V's theirs: each load has the other
-  // half of a step to arrive in, and a third more waves are resident than with a second set (whose registers would not
-  // fit three waves per SIMD at D = 128: spills, which wait for every load ahead of them). Tiles are looked up two steps
-  // ahead; those past the end are the last tile again.
+  // The registers of a step's K take the next step's as soon as they are read, and V's theirs: each load has the other half of a
+  // step to arrive in. With a second set of registers instead, waves spilled or were half as many (32 x 16384 keys: 108 and 93 us
+  // against 84). Tiles are looked up two steps ahead; those past the end are the last tile again.
   Tiles where{}, then{};
   int t0 = t_begin + wave * STEP;
   if (t0 < t_end) {
@@ -905,7 +907,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, D == 128 ? 4 : 5) void attention_i
 }
 
 // Rows of several chunks: one workgroup per (row, query, head) joins the chunks' partials, D / 4 lanes a partial, 1024 / D
-// partials at once.
+// partials at once: 4-5 us, most of it the launch (one thread per dim over 128 chunks 59).
 template <int DT, int D>
 __global__ __launch_bounds__(256) void merge_int4_kernel(Int4Attn p) {
   constexpr int LANES = D / 4, SETS = 256 / LANES;
@@ -1000,7 +1002,7 @@ void launch_attn4(const Int4Attn& p, hipStream_t stream) {
     hipLaunchKernelGGL((attention_int4_mfma_kernel<DT, D>), dim3((uint32_t)(p.batch * qtiles * p.kv_heads), p.nchunk),
                        dim3(64 * kAttnWaves), lds, stream, p, dv);
   } else {
-    hipLaunchKernelGGL((attention_int4_kernel<DT, D>), dim3(items, p.nchunk), dim3(64 * kAttnWaves), 0, stream, p);
+    hipLaunchKernelGGL((attention_int4_kernel<D>), dim3(items, p.nchunk), dim3(64 * kAttnWaves), 0, stream, p);
   }
   if (p.nchunk > 1) hipLaunchKernelGGL((merge_int4_kernel<DT, D>), dim3(items), dim3(256), 0, stream, p);
 }
