@@ -707,7 +707,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, D == 128 ? 4 : 5) void attention_i
   const int least = min(seen((int)udiv(qt * 16, dv.group)), t_end);
   // Q^T: lane (query r, g) holds 8 dims of product G.
   uint4 qf[ND], qs;
-  float c = fmaxf(fabsf(p.scale_log2), 1.17549435e-38f);  // positive, as the maximum is taken over unscaled scores
+  float c;  // of the scores; positive and finite, as the maximum is taken over unscaled ones and -infinity marks a masked key
   const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
   {
     float f[ND][8], top = 0.f;
@@ -719,7 +719,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, D == 128 ? 4 : 5) void attention_i
     }
     top = max_groups(top);
     const int ex = top > 0.f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) : 0;
-    c = ldexpf(c, ex);
+    c = fminf(fmaxf(ldexpf(fabsf(p.scale_log2), ex), 1.17549435e-38f), 3.4028234664e38f);
     // Of the group whose (scale, low) the lane's kr holds: its sum of q, and of q times the codes' bases.
     float sum = 0.f, based = 0.f;
 #pragma unroll

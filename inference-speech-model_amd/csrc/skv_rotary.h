@@ -41,8 +41,8 @@ struct RotaryAppend {
   uint32_t head_bytes;
 };
 
-// Indexes from, from + step, ... of the rows' work: one thread per pair of 16-byte vectors of one head: the two that a rotation mixes (neighbours where interleaved, rot / 2
-// apart otherwise), so a row may be rotated in place. Heads come as q, k, v.
+// Indexes from, from + step, ... of the rows' work: one thread per pair of 16-byte vectors of one head, the two that a rotation
+// mixes (neighbours where interleaved, rot / 2 apart otherwise), so a row may be rotated in place. Heads come as q, k, v.
 template <int DT, bool INTERLEAVED>
 __device__ __forceinline__ void rotate_rows(const RotaryAppend& a, uint32_t from, uint32_t step) {
   constexpr int EPL = Elt<DT>::EPL;

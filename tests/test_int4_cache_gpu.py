@@ -250,6 +250,14 @@ def test_attention_query_sizes(cuda, dtype, q_scale):
     run_attention(2, 1, 4, 2, 64, 16, [90, 31], dtype, False, q_scale=q_scale, scale=1.0 / (8 * max(q_scale, 1.0)))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_scale_zero_and_tiny_queries(cuda, dtype):
+    """Keys past a row's end stay out when scale and queries together leave fp32's range below: the mean of the values."""
+    tiny = 2.0 ** -100 if dtype == torch.bfloat16 else 2.0 ** -14
+    run_attention(3, 2, 4, 2, 64, 16, [90, 31, 1], dtype, True, scale=0.0, q_scale=tiny)
+    run_attention(3, 1, 4, 2, 64, 16, [90, 31, 0], dtype, False, scale=1e-30, q_scale=tiny)
+
+
 def test_attention_long_row(cuda):
     run_attention(1, 1, 8, 2, 128, 16, [9001], torch.bfloat16, False)
 
