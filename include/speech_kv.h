@@ -472,8 +472,8 @@ SKV_API int skv_append_rotary(const void* q, int64_t q_stride_n, int64_t q_strid
  *   Each 32 consecutive dims of a (token, head) row share fp16 (scale, low); an element is low + scale * code, code 0..15:
  *   low = fp16(min), scale = fp16(max(0, (max - low) / 15)), code = round((x - low) * (1 / scale)) clamped (0 where scale
  *   is 0), in fp32. Values beyond +-16384 saturate and a NaN is held as 0.
- *   Pools: uint8 [num_blocks, kv heads, block_size / 16, 10 * D], block_size a multiple of 16, D in {32, 64, 128}. The
- *   16-token tile of a K pool is [16 tokens][D / 2] bytes, a dword per 8 dims with dims 0..7 in nibbles 0, 4, 1, 5, 2, 6, 3,
+ *   Pools: uint8 [num_blocks, kv heads, block_size / 16, 10 * D], block_size a multiple of 16, D in {32, 64, 128}; a block
+ *   is less than 2 GiB. The 16-token tile of a K pool is [16 tokens][D / 2] bytes, a dword per 8 dims with dims 0..7 in nibbles 0, 4, 1, 5, 2, 6, 3,
  *   7, then [16][D / 32] fp16 pairs (scale, low); of a V pool [4 quads][D / 2][4 tokens] bytes, dims 2m and 2m + 1 in the low
  *   and high nibble of byte m, then [4 quads][D / 32][scale, low][4 tokens in the order 0, 2, 1, 3] fp16.
  *   No counterpart in the reference, whose pools are 16-bit.
@@ -510,8 +510,9 @@ SKV_API int64_t skv_int4_workspace_bytes(int32_t batch, int32_t q_len, int32_t n
 /*
  * skv_paged_attention_int4 — softmax(q K^T * scale) V over the 4-bit paged cache of each row: skv_paged_attention's q, out,
  * tables, ctx_lens, max_ctx and causal (0 or SKV_ATTN_CAUSAL), without a fused append. q and out are in dtype. A query with
- * no visible key gets zeros; keys behind a block id outside the pool are left out. workspace: skv_int4_workspace_bytes, any
- * content; two launches that may overlap in time need one each.
+ * no visible key gets zeros; keys behind a block id outside the pool are left out. The slots of positions below ctx_lens hold
+ * appended rows or zeros (what any other slot holds does not count). out does not overlap q. workspace:
+ * skv_int4_workspace_bytes, any content; two launches that may overlap in time need one each.
  */
 SKV_API int skv_paged_attention_int4(const void* q, int64_t q_stride_b, int64_t q_stride_q, int64_t q_stride_h,
                                      const void* k_pool, const void* v_pool, const int32_t* block_tables,
@@ -527,7 +528,8 @@ SKV_API int skv_paged_attention_int4(const void* q, int64_t q_stride_b, int64_t 
  *   q, out [N, num_heads, D], k, v [N, num_kv_heads, D] rows at their own strides (slices of a fused projection are fine);
  *   sequence s is rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (int32 [num_seqs + 1] device, non-decreasing, within
  *   0..N), of any length, 0 included; its query i sees its keys 0..i, whatever the later keys hold. Rows of out that belong
- *   to no sequence are left as they are. head_dim in {16, 32, 64, 128}; row strides of k and v from 0 to below 16 MiB.
+ *   to no sequence are left as they are; out does not overlap q, k or v. head_dim in {16, 32, 64, 128}; row strides of k and v
+ *   from 0 to below 16 MiB.
  * Replaces, for prompts of different lengths, the padded batch of models.py:126-165.
  */
 SKV_API int skv_prompt_attention(const void* q, int64_t q_stride_n, int64_t q_stride_h, const void* k, int64_t k_stride_n,

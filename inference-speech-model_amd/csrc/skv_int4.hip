@@ -1070,6 +1070,9 @@ int check_pool(const char* who, const void* k_pool, const void* v_pool, int32_t 
     return fail(SKV_EINVAL, "%s: bad pool kv_heads=%d num_blocks=%lld block_size=%d (a multiple of %d)", who, kv_heads,
                 (long long)nb, bs, kTile);
   if (nb * (bs / kTile) > (int64_t)1 << 29) return fail(SKV_EINVAL, "%s: pool of %lld x %d tokens is too large", who, (long long)nb, bs);
+  // The attention counts a block's bytes in 32 bits.
+  if ((int64_t)kv_heads * (bs / kTile) * (10 * d) >= (int64_t)1 << 31)
+    return fail(SKV_EINVAL, "%s: a block of %d heads x %d tokens x %d dims is too large", who, kv_heads, bs, d);
   if (!k_pool || !v_pool) return fail(SKV_EINVAL, "%s: null pool", who);
   if (!aligned16(k_pool) || !aligned16(v_pool)) return fail(SKV_EALIGN, "%s: pools must be 16-byte aligned", who);
   return SKV_OK;

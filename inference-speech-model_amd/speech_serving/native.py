@@ -1239,7 +1239,8 @@ def paged_attention_int4(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     """paged_attention() over a 4-bit cache: softmax(q K^T * scale) V over the values that each row's blocks hold.
 
     q: [B, H, D] or [B, Q, H, D] in any of the three types, which is the result's; the other arguments are
-    paged_attention's. The split-K partials live in memory of this call's own, so captured graphs share none."""
+    paged_attention's; out does not overlap q. The split-K partials live in memory of this call's own, so captured graphs
+    share none."""
     what = "paged_attention_int4"
     block_tables, ctx_lens = _i32(block_tables, "block_tables"), _i32(ctx_lens, "ctx_lens")
     if table_rows is not None:
@@ -1283,7 +1284,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     query i sees its keys 0..i.
 
     q: [N, H, D]; k, v: [N, Hkv, D], H a multiple of Hkv (any row/head strides); cu_seqlens: int32 [S + 1] on the GPU. Rows of
-    out behind the last sequence (a padded batch) are left as they are; they are undefined when out is not given.
+    out behind the last sequence (a padded batch) are left as they are; they are undefined when out is not given. out does not
+    overlap q, k or v.
     Reference math: speech_serving/models.py:126-165, per prompt."""
     what = "prompt_attention"
     cu_seqlens = _i32(cu_seqlens, "cu_seqlens")

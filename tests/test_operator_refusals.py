@@ -100,6 +100,15 @@ def test_prompt_attention_entry(lib, change, code, word):
     assert rc == code and word in lib.skv_last_error(), lib.skv_last_error()
 
 
+def test_int4_blocks_past_2_gib(lib):
+    """Blocks whose bytes pass 31 bits, which the attention counts in 32, are refused by every call of the cache."""
+    big = dict(kv=256, d=128, bs=1 << 17, nb=1)  # 256 heads x 8192 tiles x 1280 bytes
+    assert lib.skv_append_int4(*{**INT4, **big}.values(), None) == EINVAL and b"block of" in lib.skv_last_error()
+    assert lib.skv_gather_int4(*{**GATHER, **big}.values(), None) == EINVAL and b"block of" in lib.skv_last_error()
+    attn = {**ATTN, **big, "heads": 256}
+    assert lib.skv_paged_attention_int4(*attn.values(), None) == EINVAL and b"block of" in lib.skv_last_error()
+
+
 def test_workspace_sizes(lib):
     assert lib.skv_int4_workspace_bytes(2, 3, 8, 64, 640, 64) == 2 * 3 * 8 * 10 * (64 + 4) * 4
     assert lib.skv_int4_workspace_bytes(2, 3, 8, 64, 64, 64) == 0
