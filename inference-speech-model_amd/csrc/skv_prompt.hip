@@ -76,7 +76,7 @@ __device__ __forceinline__ void query_slow(const PromptAttn& p, int row, int beg
 //   in both operands. V^T comes from the row-major LDS rows through the transpose load.
 // The running maximum and sum and the accumulators are fp32; the weights are rounded to the rows' type for their product
 // (by half a step each, 2^-8 or 2^-11, as the result is), their sum takes them unrounded.
-// What bounds it: the matrix cores (52 % of the clocks) and the vector operations of the softmax (36 %), which two waves per SIMD
+// What bounds it: the matrix cores (55 % of the clocks) and the vector operations of the softmax (47 %), which two waves per SIMD
 // overlap in part. bf16: 16384 tokens, 32 / 8 heads x 128, 2.07-2.2 ms (1000-1060 TFLOP/s, the library's 8192^3 product 1402);
 // 20 heads x 64 0.75-0.8 ms (870-910); 8 x 448 tokens 14.7 us.
 // ---------------------------------------------------------------------------
@@ -98,42 +98,52 @@ __device__ __forceinline__ float wave_max(float x) {
   return fmaxf(x, xor_lane<32>(x));
 }
 
-// The (sequence, query tile) of a work index: sequences have ceil(length / M) tiles each, and tiles with more keys come first
-// (within each 64 sequences), so that the workgroups that take longest do not start last. False past the last tile.
+// The (sequence, query tile) of a work index. Sequence s has its places from start(s) = floor(cu[s] / M) + s on, which leaves
+// each its ceil(length / M) tiles and takes n / M + seqs in all, so that the 64 sequences around an index are found by a search
+// over cu instead of a sum over all that come before (bf16 20 heads x 64, 1024 prompts of 30 tokens: 237 us with the sum, now
+// 157; 4096 of one token 1277, now 412). Within the 64, tiles with more keys come first, so that the workgroups that take longest do not start last. False for a
+// place without a tile.
 template <int M>
 __device__ __forceinline__ bool find_tile(const PromptAttn& p, int index, int& begin, int& len, int& tile) {
   const int lane = threadIdx.x & 63;
-  for (int s0 = 0; s0 < p.seqs; s0 += 64) {
-    int b = 0, e = 0;
-    if (s0 + lane < p.seqs) seq_range(p, s0 + lane, b, e);
-    const int n = (e - b + M - 1) / M;
-    // Tiles with a number of t or more, over the 64 sequences (fewer than 2^24 in a launch, which floats count).
-    auto from = [&](int t) __attribute__((always_inline)) {
-      return __builtin_amdgcn_readfirstlane((int)group_sum<64>((float)max(n - t, 0)));
-    };
-    const int all = from(0);
-    if (index >= all) {
-      index -= all;
-      continue;
+  int s0 = 0;
+  for (int span = (p.seqs + 63) / 64; span > 1;) {  // groups of 64 that may hold the index, from s0 on
+    const int step = (span + 63) / 64;
+    bool at_or_before = false;
+    if (lane * step < span) {
+      const int s = s0 + 64 * lane * step;
+      at_or_before = min(max(p.cu[s], 0), p.n) / M + s <= index;
     }
-    int lo = 0, hi = __builtin_amdgcn_readfirstlane((int)wave_max((float)n)), ahead = 0;
-    while (hi - lo > 1) {  // from(lo) > index >= from(hi) = ahead
-      const int mid = (lo + hi) / 2, f = from(mid);
-      if (f > index)
-        lo = mid;
-      else
-        hi = mid, ahead = f;
-    }
-    // The (index - ahead)-th sequence of those that have a tile number lo.
-    const uint64_t have = __builtin_amdgcn_ballot_w64(n > lo);
-    const int before = __builtin_popcountll(have & ((1ull << lane) - 1));
-    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(n > lo && before == index - ahead));
-    begin = __builtin_amdgcn_readlane(b, l);
-    len = __builtin_amdgcn_readlane(e, l) - begin;
-    tile = lo;
-    return true;
+    const int last = __builtin_popcountll(__builtin_amdgcn_ballot_w64(at_or_before)) - 1;
+    if (last < 0) return false;
+    s0 += 64 * last * step;
+    span = min(step, span - last * step);
   }
-  return false;
+  int b = 0, e = 0;
+  if (s0 + lane < p.seqs) seq_range(p, s0 + lane, b, e);
+  index -= __builtin_amdgcn_readfirstlane(b) / M + s0;
+  const int n = (e - b + M - 1) / M;
+  // Tiles with a number of t or more, over the 64 sequences (fewer than 2^24 in a launch, which floats count).
+  auto from = [&](int t) __attribute__((always_inline)) {
+    return __builtin_amdgcn_readfirstlane((int)group_sum<64>((float)max(n - t, 0)));
+  };
+  if (index < 0 || index >= from(0)) return false;
+  int lo = 0, hi = __builtin_amdgcn_readfirstlane((int)wave_max((float)n)), ahead = 0;
+  while (hi - lo > 1) {  // from(lo) > index >= from(hi) = ahead
+    const int mid = (lo + hi) / 2, f = from(mid);
+    if (f > index)
+      lo = mid;
+    else
+      hi = mid, ahead = f;
+  }
+  // The (index - ahead)-th sequence of those that have a tile number lo.
+  const uint64_t have = __builtin_amdgcn_ballot_w64(n > lo);
+  const int before = __builtin_popcountll(have & ((1ull << lane) - 1));
+  const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(n > lo && before == index - ahead));
+  begin = __builtin_amdgcn_readlane(b, l);
+  len = __builtin_amdgcn_readlane(e, l) - begin;
+  tile = lo;
+  return true;
 }
 
 template <int DT, int D, int QW, int KW>

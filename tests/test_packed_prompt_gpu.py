@@ -76,6 +76,29 @@ def test_many_sequences(cuda):
     check(out, q, k, v, lens, 0.125)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_thousands_of_sequences(cuda, dtype):
+    """More groups of 64 sequences than a wave has lanes, empty sequences among them, long ones first, in between and last;
+    against one float64 softmax under the sequences' mask, with reference()'s bound."""
+    lens = [500] + [(7 * i) % 4 for i in range(2500)] + [260] + [(5 * i) % 3 for i in range(2500)] + [130]
+    n, h, hkv, d, scale = sum(lens), 2, 1, 64, 0.125
+    q, k, v = inputs(n, h, hkv, d, dtype)
+    out = native.prompt_attention(q, k, v, cumulative(lens), scale)
+    seq = torch.repeat_interleave(torch.arange(len(lens), device="cuda"), torch.tensor(lens, device="cuda"))
+    seen = (seq[:, None] == seq[None, :]).tril()
+    kk, vv, half = k[:, 0].double(), v[:, 0].double(), ic.half_step(dtype)
+    for i in range(h):
+        qq = q[:, i].double()
+        s = ((qq @ kk.T) * scale).masked_fill(~seen, -math.inf)
+        w = torch.softmax(s, -1)
+        ds = scale * (d + 8) * 2.0 ** -24 * (qq.abs() @ kk.abs().T) + 2.0 ** -21 * s.abs() + 2.0 ** -21
+        ds = torch.where(seen, ds, torch.zeros_like(ds)).amax(-1, keepdim=True)
+        o, absw = w @ vv, w @ vv.abs()
+        weights = 0.0 if dtype == torch.float32 else half
+        bound = (weights + torch.expm1(2 * ds) + 2.0 ** -20) * (absw + o.abs()) + half * o.abs() + 2.0 ** -25
+        assert ((out[:, i].double() - o).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("scale", [0.0, -0.2, 2.0])
 def test_scales(cuda, dtype, scale):
