@@ -69,7 +69,7 @@ __device__ __forceinline__ void query_slow(const PromptAttn& p, int row, int beg
 
 // ---------------------------------------------------------------------------
 // 16-bit rows on the matrix cores: one workgroup owns 32 * QW consecutive queries of one head, 32 per wave, and walks the keys
-// up to its last query in tiles of 64 staged in LDS (double-buffered, one barrier per tile). KW = 2: two waves share 32 queries,
+// up to its last query in tiles of KT staged in LDS (double-buffered, one barrier per tile). KW = 2: two waves share 32 queries,
 // each with half of every tile's keys, and join at the end.
 //   S^T = K Q^T in 32 x 32 products: a lane holds 16 keys' scores of one query per product, whose softmax weights are, in
 //   place, the operand of O^T = V^T P^T: contraction element (half f, j) of a 16-key step stands for key 4 f + j, 8 + 4 f + j - 4
@@ -80,7 +80,6 @@ __device__ __forceinline__ void query_slow(const PromptAttn& p, int row, int beg
 // overlap in part. bf16: 16384 tokens, 32 / 8 heads x 128, 2.07-2.2 ms (1000-1060 TFLOP/s, the library's 8192^3 product 1402);
 // 20 heads x 64 0.75-0.8 ms (870-910); 8 x 448 tokens 14.7 us.
 // ---------------------------------------------------------------------------
-constexpr int kKeys = 64;            // keys of a staged tile
 constexpr float kLazyMaxLog2 = 8.f;  // the accumulators are rescaled when a maximum grows by more than this
 
 typedef short v4i16 __attribute__((ext_vector_type(4)));
@@ -100,8 +99,8 @@ __device__ __forceinline__ float wave_max(float x) {
 
 // The (sequence, query tile) of a work index. Sequence s has its places from start(s) = floor(cu[s] / M) + s on, which leaves
 // each its ceil(length / M) tiles and takes n / M + seqs in all, so that the 64 sequences around an index are found by a search
-// over cu instead of a sum over all that come before (bf16 20 heads x 64, 1024 prompts of 30 tokens: 237 us with the sum, now
-// 157; 4096 of one token 1277, now 412). Within the 64, tiles with more keys come first, so that the workgroups that take longest do not start last. False for a
+// over cu instead of a sum over all that come before (128 queries a workgroup, bf16 20 heads x 64, 1024 prompts of 30 tokens:
+// 237 us with the sum, 157 with the search; 4096 of one token 1277 and 412). Within the 64, tiles with more keys come first, so that the workgroups that take longest do not start last. False for a
 // place without a tile.
 template <int M>
 __device__ __forceinline__ bool find_tile(const PromptAttn& p, int index, int& begin, int& len, int& tile) {
@@ -146,19 +145,19 @@ __device__ __forceinline__ bool find_tile(const PromptAttn& p, int index, int& b
   return true;
 }
 
-template <int DT, int D, int QW, int KW>
+template <int DT, int D, int QW, int KW, int KT>
 __global__ __launch_bounds__(64 * QW * KW, 2) void prompt_kernel(PromptAttn p) {
   constexpr int M = 32 * QW;
-  constexpr int KB = 2 / KW;                // 32-key blocks of a tile that a wave takes
+  constexpr int KB = KT / 32 / KW;          // 32-key blocks of a tile that a wave takes
   constexpr int VPR = D / 8;                // 16-byte vectors per row
   constexpr int RPP = 64 * QW * KW / VPR;   // rows a pass of the workgroup loads
-  constexpr int PASSES = RPP > kKeys ? 1 : kKeys / RPP;
+  constexpr int PASSES = RPP > KT ? 1 : KT / RPP;
   // LDS rows are padded so that neither the 16 rows of a K load (16 bytes each) nor the 4 rows of a V^T load (64 bytes each)
   // meet in a bank.
   constexpr int KROW = D * 2 + 16, VROW = D * 2 + (D == 32 ? 0 : 64);
   constexpr int KS = D / 16;                // contraction steps of a score product
   constexpr int DB = D / 32;                // 32-dim blocks of the result
-  constexpr int KBUF = kKeys * KROW, VBUF = kKeys * VROW;
+  constexpr int KBUF = KT * KROW, VBUF = KT * VROW;
   constexpr int JOIN = KW == 1 ? 0 : QW * 64 * (16 * DB + 2) * 4;  // the second key half's state
   constexpr int LDS = 2 * (KBUF + VBUF) > JOIN ? 2 * (KBUF + VBUF) : JOIN;
   __shared__ __attribute__((aligned(16))) char s_mem[LDS];
@@ -197,7 +196,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void prompt_kernel(PromptAttn p) {
   const char* kbase = p.k + (int64_t)begin * p.ksn + (int64_t)kvh * p.ksh;
   const char* vbase = p.v + (int64_t)begin * p.vsn + (int64_t)kvh * p.vsh;
   const int ld_row = threadIdx.x / VPR, ld_col = (threadIdx.x % VPR) * 16;
-  const bool loads = ld_row < kKeys;  // with D = 32 a pass may hold more rows than a tile
+  const bool loads = ld_row < KT;  // with D = 32 a pass may hold more rows than a tile
   uint4 kr[PASSES], vr[PASSES];
   // Byte offsets of the lane's vectors within a tile; head_dim 16 leaves the upper half of 32 dims zeros.
   uint32_t koff[PASSES], voff[PASSES];
@@ -211,7 +210,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void prompt_kernel(PromptAttn p) {
   auto issue = [&](const char* base, int64_t stride, int t0, const uint32_t (&off)[PASSES], uint4 (&r)[PASSES])
                    __attribute__((always_inline)) {
     const int left = len - t0;  // may be 0 or less: nothing is read
-    const int64_t bytes = left > 0 ? (int64_t)(min(left, kKeys) - 1) * stride + p.row_bytes : 0;
+    const int64_t bytes = left > 0 ? (int64_t)(min(left, KT) - 1) * stride + p.row_bytes : 0;
     const __amdgpu_buffer_rsrc_t res =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + (int64_t)t0 * stride), (short)0, (int)bytes, kBufWord3);
 #pragma unroll
@@ -259,22 +258,22 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void prompt_kernel(PromptAttn p) {
   issue_k(0);
   issue_v(0);
   stage_k(0);
-  issue_k(kKeys);
+  issue_k(KT);
   __syncthreads();
   f32x16 s[KB], s_next[KB];
   scores(0, s);
   stage_v(0);
   stage_k(1);
-  issue_k(2 * kKeys);
-  issue_v(kKeys);
+  issue_k(2 * KT);
+  issue_v(KT);
   lds_barrier();
-  for (int t0 = 0, buf = 0; t0 < keys; t0 += kKeys, buf ^= 1) {
+  for (int t0 = 0, buf = 0; t0 < keys; t0 += KT, buf ^= 1) {
     // Tile t0 + 128's K goes where tile t0's was, tile t0 + 64's V where tile t0 - 64's was: the last barrier is behind their reads.
     if (t0 > 0) {
       stage_v(buf);
       stage_k(buf ^ 1);
-      issue_k(t0 + 2 * kKeys);
-      issue_v(t0 + kKeys);
+      issue_k(t0 + 2 * KT);
+      issue_v(t0 + KT);
       lds_barrier();
     }
     const int k0 = t0 + 32 * KB * kw;  // the wave's first key of the tile
@@ -366,7 +365,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void prompt_kernel(PromptAttn p) {
     for (int i = 0; i < 16; ++i) all += fabsf(acc[db][i]);
   if (__builtin_amdgcn_ballot_w64(!(all < __builtin_huge_valf())) != 0) {
     bool bad = false;
-    for (int t = first; t < min(len, (wave_keys + kKeys - 1) / kKeys * kKeys); ++t) {
+    for (int t = first; t < min(len, (wave_keys + KT - 1) / KT * KT); ++t) {
       const elt_t<DT>* v = reinterpret_cast<const elt_t<DT>*>(vbase + (int64_t)t * p.vsn);
       for (int d = lane; 2 * d < p.row_bytes; d += 64) bad |= !(fabsf((float)v[d]) < __builtin_huge_valf());
     }
@@ -514,20 +513,27 @@ __global__ __launch_bounds__(64 * kWaves32) void prompt_f32_kernel(PromptAttn p)
   for (int qi = first + wave; qi < keys; qi += kWaves32) query_slow<SKV_F32, D>(p, begin + qi, begin, h);
 }
 
-template <int DT, int D, int QW, int KW>
+template <int DT, int D, int QW, int KW, int KT>
 void launch_tiles(const PromptAttn& p, hipStream_t stream) {
   const int tiles = p.n / (32 * QW) + p.seqs;  // at least the sum of ceil(length / M)
-  hipLaunchKernelGGL((prompt_kernel<DT, D, QW, KW>), dim3((uint32_t)tiles * (uint32_t)p.heads), dim3(64 * QW * KW), 0, stream, p);
+  hipLaunchKernelGGL((prompt_kernel<DT, D, QW, KW, KT>), dim3((uint32_t)tiles * (uint32_t)p.heads), dim3(64 * QW * KW), 0, stream, p);
 }
-// Few workgroups (no more than the compute units) are as slow as the one with the most keys: two waves then share 32 queries'
-// keys. bf16 32 / 8 heads x 128 (us, 128 queries a workgroup / 64 with shared keys): 512 tokens (128 workgroups) 15.9 / 12.3,
-// 2048 tokens (512) 52 / 54, 16384 tokens 2070 / 2450; 20 heads x 64, 8 x 448 tokens (640) 18.1 / 18.3.
+// Three forms, by what the host knows: rows, sequences and heads. bf16, us of the form with 128 queries / the one named:
+//   Short sequences, up to 128 rows on average: 64 queries a workgroup and 32 keys a tile, whose small LDS lets more
+//     workgroups run at once, each with less padding. 20 heads x 64: 1024 x 30 tokens 157 / 98, 256 x 60 43 / 35, 256 x 120
+//     90 / 90, 64 x 200 40 / 46; 32 / 8 heads x 128: 256 x 60 139 / 105, 2048 and 200 x 10 105 / 74, 2048..1 (16) 80 / 82.
+//   Few workgroups (no more than the compute units) are as slow as the one with the most keys: two waves share 32 queries'
+//     keys. 32 / 8 heads x 128: 512 tokens (128 workgroups) 15.9 / 12.4, 2048 tokens (512) 53 / 55; 20 heads x 64: 100 tokens
+//     6.0 / 5.1 (the short form 5.6), 8 x 48 4.7 / 4.6 (4.7), 8 x 30 4.3 / 4.3 (3.8): the short form up to 64 on average.
 template <int DT, int D>
 void launch_prompt(const PromptAttn& p, hipStream_t stream) {
-  if (cdiv(p.n, 128) * p.heads <= compute_units())
-    launch_tiles<DT, D, 2, 2>(p, stream);
+  const bool few = cdiv(p.n, 128) * p.heads <= compute_units();
+  if (p.n <= (few ? 64 : 128) * (int64_t)p.seqs)
+    launch_tiles<DT, D, 2, 1, 32>(p, stream);
+  else if (few)
+    launch_tiles<DT, D, 2, 2, 64>(p, stream);
   else
-    launch_tiles<DT, D, 4, 1>(p, stream);
+    launch_tiles<DT, D, 4, 1, 64>(p, stream);
 }
 template <int D>
 void launch_prompt_f32(const PromptAttn& p, hipStream_t stream) {

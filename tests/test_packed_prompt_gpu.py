@@ -76,6 +76,28 @@ def test_many_sequences(cuda):
     check(out, q, k, v, lens, 0.125)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("lens,h,hkv", [([900, 417, 70], 32, 8), ([700, 30], 4, 2), ([20] * 70 + [333, 65], 4, 2)])
+def test_forms(cuda, dtype, d, lens, h, hkv):
+    """Many workgroups of long sequences, few, and short sequences beside a long one; then the same with a NaN row in the
+    first long sequence, which only its later queries may see."""
+    q, k, v = inputs(sum(lens), h, hkv, d, dtype)
+    scale = 1 / math.sqrt(d)
+    out = native.prompt_attention(q, k, v, cumulative(lens), scale)
+    check(out, q, k, v, lens, scale)
+    i = lens.index(max(lens))
+    at, n, bad = sum(lens[:i]), lens[i], 3 * lens[i] // 5
+    k2, v2 = k.clone(), v.clone()
+    k2[at + bad, 0], v2[at + bad, -1, 5] = math.nan, math.inf
+    got = native.prompt_attention(q, k2, v2, cumulative(lens), scale)
+    first = slice(at, at + bad)
+    check(got[first], q[first], k[first], v[first], [bad], scale)
+    assert torch.equal(got[:at], out[:at]) and torch.equal(got[at + n:], out[at + n:])
+    group = h // hkv
+    assert torch.isnan(got[at + bad:at + n, :group]).all() and not torch.isfinite(got[at + bad:at + n, -group:, 5]).any()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_thousands_of_sequences(cuda, dtype):
     """More groups of 64 sequences than a wave has lanes, empty sequences among them, long ones first, in between and last;
