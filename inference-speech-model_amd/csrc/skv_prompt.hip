@@ -522,12 +522,13 @@ void launch_tiles(const PromptAttn& p, hipStream_t stream) {
 //   Short sequences, up to 128 rows on average: 64 queries a workgroup and 32 keys a tile, whose small LDS lets more
 //     workgroups run at once, each with less padding. 20 heads x 64: 1024 x 30 tokens 157 / 98, 256 x 60 43 / 35, 256 x 120
 //     90 / 90, 64 x 200 40 / 46; 32 / 8 heads x 128: 256 x 60 139 / 105, 2048 and 200 x 10 105 / 74, 2048..1 (16) 80 / 82.
-//   Few workgroups (no more than the compute units) are as slow as the one with the most keys: two waves share 32 queries'
-//     keys. 32 / 8 heads x 128: 512 tokens (128 workgroups) 15.9 / 12.4, 2048 tokens (512) 53 / 55; 20 heads x 64: 100 tokens
-//     6.0 / 5.1 (the short form 5.6), 8 x 48 4.7 / 4.6 (4.7), 8 x 30 4.3 / 4.3 (3.8): the short form up to 64 on average.
+//   Few workgroups of 128 (up to 1.5 a compute unit; two fit on one) are as slow as the one with the most keys: two waves share
+//     32 queries' keys. Heads x 128: 32 x 512 tokens (128 workgroups) 15.9 / 12.4, 8 x 4096 (256) 81 / 61, 6 x 6428 (306) 126 / 95,
+//     20 x 3 prompts of 700 (340) 22 / 24, 12 x 4096 (384) 88 / 76, 28 x 2048 (448) 51 / 53, 32 x 2048 (512) 53 / 55; x 64: 20 x
+//     2048 (320) 32 / 24, 20 x 100 6.0 / 5.1 (the short form 5.6), 20 x 8 of 30 4.3 / 4.3 (3.8): the short form up to 64 on average.
 template <int DT, int D>
 void launch_prompt(const PromptAttn& p, hipStream_t stream) {
-  const bool few = cdiv(p.n, 128) * p.heads <= compute_units();
+  const bool few = 2 * cdiv(p.n, 128) * p.heads <= 3 * compute_units();
   if (p.n <= (few ? 64 : 128) * (int64_t)p.seqs)
     launch_tiles<DT, D, 2, 1, 32>(p, stream);
   else if (few)

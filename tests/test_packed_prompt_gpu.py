@@ -78,9 +78,9 @@ def test_many_sequences(cuda):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", [16, 32, 64, 128])
-@pytest.mark.parametrize("lens,h,hkv", [([900, 417, 70], 32, 8), ([700, 30], 4, 2), ([20] * 70 + [333, 65], 4, 2)])
+@pytest.mark.parametrize("lens,h,hkv", [([1500, 417, 70], 40, 8), ([900, 417, 70], 32, 8), ([700, 30], 4, 2), ([20] * 70 + [333, 65], 4, 2)])
 def test_forms(cuda, dtype, d, lens, h, hkv):
-    """Many workgroups of long sequences, few, and short sequences beside a long one; then the same with a NaN row in the
+    """Many workgroups of long sequences, fewer, few, and short sequences beside a long one; then the same with a NaN row in the
     first long sequence, which only its later queries may see."""
     q, k, v = inputs(sum(lens), h, hkv, d, dtype)
     scale = 1 / math.sqrt(d)
