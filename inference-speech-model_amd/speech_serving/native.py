@@ -1120,7 +1120,7 @@ def _append_rows(what: str, k_new, v_new, k_pool, v_pool, slot_mapping, position
         q, qn, qh = _rows3(what, q, "q", q_shape, dt)
         q_args = (q.data_ptr(), qn, qh)
         if q_out is None:
-            q_out = torch.empty(q_shape, dtype=dt, device=q.device)
+            q_out = q.new_empty(q_shape)
             qo_args = (q_out.data_ptr(), heads * shape[2], shape[2])
         else:
             _, qn, qh = _rows3(what, q_out, "q_out", q_shape, dt, written=True)
@@ -1224,6 +1224,16 @@ def gather_int4(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.
     return outs[0], outs[1]
 
 
+def _dims4(t: torch.Tensor, name: str) -> Tuple[int, ...]:
+    """(B, Q, H, D and their strides) of a [B, Q, H, D] or, Q being 1, [B, H, D] tensor: _q4 without a view."""
+    if t.dim() == 3:
+        (b, h, d), (sb, sh, sd) = t.shape, t.stride()
+        return b, 1, h, d, sb, 0, sh, sd
+    if t.dim() == 4:
+        return (*t.shape, *t.stride())
+    raise RuntimeError(f"{name} must be [B, H, D] or [B, Q, H, D], got {tuple(t.shape)}")
+
+
 @functools.lru_cache(maxsize=4096)
 def _int4_plan(batch: int, q_len: int, heads: int, kv_heads: int, head_dim: int, max_ctx: int, code: int,
                chunk: int) -> Tuple[int, int]:
@@ -1247,8 +1257,7 @@ def paged_attention_int4(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
         table_rows = _i32(table_rows, "table_rows")
     dev = _one_device(what, q, k_pool, v_pool, block_tables, ctx_lens, table_rows, out)
     nb, bs, hkv, dk = _int4_pools(what, k_pool, v_pool)
-    q4 = _q4(q, "q")
-    bsz, qlen, heads, d = q4.shape
+    bsz, qlen, heads, d, qb, qq, qh, qd = _dims4(q, "q")
     if d != dk or heads % hkv:
         raise RuntimeError(f"{what}: {heads} heads x {d} do not fit pools of {hkv} heads x {dk}")
     if block_tables.dim() != 2 or ctx_lens.numel() < bsz:
@@ -1259,21 +1268,21 @@ def paged_attention_int4(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
         raise RuntimeError(f"{what}: table_rows must cover the batch")
     code = _code(q.dtype)
     wide = 3 if q.dtype is torch.float32 else 7
-    qb, qq, qh, qd = q4.stride()
-    if qd != 1 or (qb | qq | qh) & wide or q4.data_ptr() & 15:
-        q4 = q4.clone(memory_format=torch.contiguous_format)
-        qb, qq, qh, _ = q4.stride()
+    if qd != 1 or (qb | qq | qh) & wide or q.data_ptr() & 15:
+        q = q.clone(memory_format=torch.contiguous_format)
+        qb, qq, qh = _dims4(q, "q")[4:7]
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    o4 = _q4(out, "out")
-    ob, oq, oh, od = o4.stride()
-    if o4.shape != q4.shape or od != 1 or out.dtype != q.dtype:
-        raise RuntimeError(f"{what}: out must match q's shape and type with contiguous head_dim")
+        out = q.new_empty(q.shape)
+        ob, oq, oh = qlen * heads * d, heads * d, d
+    else:
+        *shape, ob, oq, oh, od = _dims4(out, "out")
+        if shape != [bsz, qlen, heads, d] or od != 1 or out.dtype != q.dtype:
+            raise RuntimeError(f"{what}: out must match q's shape and type with contiguous head_dim")
     max_ctx = max(0, min(int(max_ctx), block_tables.shape[1] * bs))
     chunk, need = _int4_plan(bsz, qlen, heads, hkv, d, max_ctx, code, int(chunk_tokens))
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _call("skv_paged_attention_int4", dev, q4.data_ptr(), qb, qq, qh, k_pool.data_ptr(), v_pool.data_ptr(),
-          block_tables.data_ptr(), block_tables.shape[1], _ptr(table_rows), ctx_lens.data_ptr(), o4.data_ptr(), ob, oq, oh, bsz,
+    _call("skv_paged_attention_int4", dev, q.data_ptr(), qb, qq, qh, k_pool.data_ptr(), v_pool.data_ptr(),
+          block_tables.data_ptr(), block_tables.shape[1], _ptr(table_rows), ctx_lens.data_ptr(), out.data_ptr(), ob, oq, oh, bsz,
           qlen, heads, hkv, d, bs, nb, max_ctx, scale, SKV_ATTN_CAUSAL if causal else 0, code, chunk, _ptr(ws), need)
     return out
 
@@ -1302,7 +1311,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     k, kn, kh = _rows3(what, k, "k", (n, hkv, d), dt)
     v, vn, vh = _rows3(what, v, "v", (n, hkv, d), dt)
     if out is None:
-        out = torch.empty((n, heads, d), dtype=dt, device=q.device)
+        out = q.new_empty((n, heads, d))
         on, oh = heads * d, d
     else:
         _, on, oh = _rows3(what, out, "out", (n, heads, d), dt, written=True)
