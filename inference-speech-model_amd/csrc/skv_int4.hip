@@ -212,7 +212,8 @@ __global__ __launch_bounds__(256) void append_int4_kernel(Int4Append a, RotaryAp
     // Whether the 4 tokens go to the 4 places of one quad in their order.
     const uint32_t key = stored && ((uint32_t)slot & 3u) == (uint32_t)k ? (uint32_t)(slot >> 2) : ~(uint32_t)k;
     const uint32_t key2 = xor_bits<2 * LPR>(key);
-    const bool whole = key == key2 && key == xor_bits<LPR>(key) && key == xor_bits<LPR>(key2);
+    const uint32_t key1 = xor_bits<LPR>(key), key3 = xor_bits<LPR>(key2);  // in all lanes: an && would leave some out
+    const bool whole = key == key1 && key == key2 && key == key3;
     if (!stored) continue;
     // slot = (block * tiles + tile of the block) * 16 + token; a (block, head) has tiles.d tiles.
     const uint32_t tile = (uint32_t)(slot >> 4);

@@ -1,5 +1,6 @@
 """The 4-bit cache: appended bytes and gathered values against numpy bit for bit, attention against float64 within the
 bounds that its roundings give."""
+import itertools
 import math
 
 import numpy as np
@@ -62,6 +63,38 @@ def test_append_order(cuda, dtype):
         kp, vp = pools(2, bs, h, d)
         native.append_int4(k[order].contiguous(), v[order].contiguous(), kp, vp, torch.tensor(at, device="cuda")[order])
         assert np.array_equal(kp.cpu().numpy(), want[0]) and np.array_equal(vp.cpu().numpy(), want[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_append_quads(cuda, dtype, d):
+    """Four consecutive rows, each at its own place of one quad, at that place or another one of a quad elsewhere, or skipped, in
+    all combinations (where one prompt ends and the next begins, some of them)."""
+    at = []
+    for i, kinds in enumerate(itertools.product(range(4), repeat=4)):
+        for k, kind in enumerate(kinds):
+            far = 1024 + 4 * (4 * i + k)
+            at.append((4 * i + k, far + k, far + (k + 1) % 4, -1)[kind])
+    n, bs, blocks = len(at), 64, 80
+    k, v = rows(n, 1, d, dtype, 1), rows(n, 1, d, dtype, 2)
+    kp, vp = pools(blocks, bs, 1, d, 0x5a)
+    native.append_int4(k, v, kp, vp, torch.tensor(at, device="cuda"))
+    for got, want in zip((kp, vp), written(k, v, at, blocks, bs, 0x5a)):
+        assert np.array_equal(got.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("lens", [[55, 55, 55], [3, 3, 2, 7], [1, 2, 3, 1], [18, 21, 47]])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_append_prompts_side_by_side(cuda, d, lens):
+    """Packed prompts of any length, each from position 0 of its own blocks on."""
+    bs, width = 16, -(-max(lens) // 16)
+    at = [(i * width) * bs + t for i, n in enumerate(lens) for t in range(n)]
+    blocks = width * len(lens)
+    k, v = rows(len(at), 2, d, torch.bfloat16, 1), rows(len(at), 2, d, torch.bfloat16, 2)
+    kp, vp = pools(blocks, bs, 2, d)
+    native.append_int4(k, v, kp, vp, torch.tensor(at, device="cuda"))
+    for got, want in zip((kp, vp), written(k, v, at, blocks, bs)):
+        assert np.array_equal(got.cpu().numpy(), want)
 
 
 def test_append_extremes(cuda):
