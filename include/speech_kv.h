@@ -470,12 +470,13 @@ SKV_API int skv_append_rotary(const void* q, int64_t q_stride_n, int64_t q_strid
 /*
  * The 4-bit paged cache (skv_append_int4, skv_gather_int4, skv_paged_attention_int4): 5 bits an element.
  *   Each 32 consecutive dims of a (token, head) row share fp16 (scale, low); an element is low + scale * code, code 0..15:
- *   low = fp16(min), scale = fp16(max(0, (max - low) / 15)), code = round((x - low) * (1 / scale)) clamped (0 where scale
+ *   low = fp16(min), scale = fp16(max(0, (max - low) * (1 / 15))), code = round((x - low) * (1 / scale)) clamped (0 where scale
  *   is 0), in fp32. Values beyond +-16384 saturate and a NaN is held as 0.
  *   Pools: uint8 [num_blocks, kv heads, block_size / 16, 10 * D], block_size a multiple of 16, D in {32, 64, 128}; a block
- *   is less than 2 GiB. The 16-token tile of a K pool is [16 tokens][D / 2] bytes, a dword per 8 dims with dims 0..7 in nibbles 0, 4, 1, 5, 2, 6, 3,
- *   7, then [16][D / 32] fp16 pairs (scale, low); of a V pool [4 quads][D / 2][4 tokens] bytes, dims 2m and 2m + 1 in the low
- *   and high nibble of byte m, then [4 quads][D / 32][scale, low][4 tokens in the order 0, 2, 1, 3] fp16.
+ *   is less than 2 GiB. The 16-token tile of a K pool is [16 tokens][D / 2] bytes, a dword per 8 dims with dims 0..7 in
+ *   nibbles 0, 4, 1, 5, 2, 6, 3, 7, then [16][D / 32] fp16 pairs (scale, low); of a V pool [4 quads][D / 2][4 tokens] bytes,
+ *   dims 2m and 2m + 1 in the low and high nibble of byte m, then [4 quads][D / 32][scale, low][4 tokens in the order 0, 2,
+ *   1, 3] fp16.
  *   No counterpart in the reference, whose pools are 16-bit.
  *
  * skv_append_int4 — K/V rows quantised into their slots, rotated first when cos_sin is given (then as skv_append_rotary, q,

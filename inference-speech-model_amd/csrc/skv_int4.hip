@@ -1,7 +1,7 @@
 // The paged 4-bit K/V cache: append (with the position rotation on the way), gather, attention.
 //
 // Format. Each 32 consecutive dims of a (token, head) row share fp16 (scale, low); an element is low + scale * code with
-// code = round((x - low) / scale) in 0..15, low = fp16(min x), scale = fp16((max x - low) / 15): 5 bits an element. Values
+// code = round((x - low) / scale) in 0..15, low = fp16(min x), scale = fp16((max x - low) * (1 / 15)): 5 bits an element. Values
 // beyond +-16384 saturate and a NaN is held as 0, so that everything the cache can hold is finite.
 // Pools are uint8 [num_blocks, kv heads, block_size / 16, 10 * D]: a head's 16-token tiles lie one after the other, so a
 // workgroup that reads one head reads whole cache lines (rows of 16 to 64 bytes per (token, head), as the 16-bit pools lay
@@ -85,13 +85,8 @@ __device__ __forceinline__ float rounded_sum(float a, float b) {
 #pragma clang fp contract(off)
   return a + b;
 }
-// x / 15, correctly rounded (the residual of a quotient that is off by an ulp at most, times the rounded reciprocal:
-// Markstein's correction), where the result is not subnormal; fp16 makes zero of those.
-__device__ __forceinline__ float div15(float x) {
-  const float q = x * (1.f / 15.f);
-  return fmaf(fmaf(-15.f, q, x), 1.f / 15.f, q);
-}
-// 1 / s of an fp16 value, correctly rounded the same way (held against the division for every fp16 number).
+// 1 / s of an fp16 value, correctly rounded: the residual of a reciprocal that is off by an ulp at most, times it (held against
+// the division for every fp16 number).
 __device__ __forceinline__ float reciprocal(float s) {
   const float r = __builtin_amdgcn_rcpf(s);
   return fmaf(fmaf(-s, r, 1.f), r, r);
@@ -182,7 +177,7 @@ __global__ __launch_bounds__(256) void append_int4_kernel(Int4Append a, RotaryAp
     hi = max_score(hi, xor_lane<2>(hi));
     const uint32_t low_h = to_half_bits(lo);
     const float low = half_bits(low_h);
-    const uint32_t scale_h = to_half_bits(fmaxf(div15(hi - low), 0.f));
+    const uint32_t scale_h = to_half_bits(fmaxf((hi - low) * (1.f / 15.f), 0.f));
     const float scale = half_bits(scale_h);
     const float inv = scale > 0.f ? reciprocal(scale) : 0.f;
     // round((x - low) / scale) in the low bits of 1.5 * 2^23 + it, clamped there as integers; words of 8 are sums, the constant

@@ -16,7 +16,7 @@ def quantise(x):
     x = np.where(np.isnan(x), np.float32(0), np.clip(x, -LIMIT, LIMIT)).astype(np.float32)
     g = x.reshape(*x.shape[:-1], -1, GROUP)
     low = g.min(-1).astype(np.float16)
-    span = (g.max(-1) - low.astype(np.float32)) / np.float32(15)
+    span = (g.max(-1) - low.astype(np.float32)) * (np.float32(1) / np.float32(15))
     scale = np.maximum(span, np.float32(0)).astype(np.float16)
     with np.errstate(divide="ignore"):
         inv = np.where(scale > 0, np.float32(1) / scale.astype(np.float32), np.float32(0)).astype(np.float32)

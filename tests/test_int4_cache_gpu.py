@@ -123,7 +123,7 @@ def test_append_extremes(cuda):
 
 def test_append_every_scale(cuda):
     """Groups of every fp16 scale up to the greatest the cache takes, its codes' borders among the elements: what the kernel's
-    quotient and reciprocal give is what division gives."""
+    reciprocal gives is what division gives."""
     scales = np.arange(1, 0x7c00, dtype=np.uint16).view(np.float16).astype(np.float32)
     scales = scales[scales <= 2184]
     n = -(-len(scales) // 8)
@@ -142,6 +142,20 @@ def test_append_every_scale(cuda):
     table = torch.arange(blocks, dtype=torch.int32, device="cuda").view(1, -1)
     for got in native.gather_int4(kp, vp, table, torch.tensor([n], dtype=torch.int32, device="cuda"), n, torch.float32):
         assert torch.equal(got[0].transpose(0, 1).cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_append_many_groups(cuda, dtype):
+    """262144 groups, enough for ranges next to a border between two fp16 scales: the product with 1 / 15 decides there."""
+    n, h, d, bs = 16384, 8, 64, 64
+    k, v = rows(n, h, d, dtype, 1), rows(n, h, d, dtype, 2, 30.0)
+    kp, vp = pools(n // bs, bs, h, d)
+    native.append_int4(k, v, kp, vp, torch.arange(n, device="cuda"))
+    table = torch.arange(n // bs, dtype=torch.int32, device="cuda").view(1, -1)
+    got = native.gather_int4(kp, vp, table, torch.tensor([n], dtype=torch.int32, device="cuda"), n, torch.float32)
+    for x, y in zip(got, (k, v)):
+        want = torch.from_numpy(ic.values(*ic.quantise(y.float().cpu().numpy()))).float()
+        assert torch.equal(x[0].transpose(0, 1).cpu(), want)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
